@@ -1,0 +1,262 @@
+// C ABI of the operators on rows grouped by the weights they use: argument
+// checks, tile planning and dispatch. No exceptions cross this boundary.
+#include "../../include/qlinear.h"
+
+#include <hip/hip_runtime.h>
+
+#include <climits>
+#include <cstdarg>
+#include <cstdint>
+#include <cstdio>
+
+#include "qlin_internal.hpp"
+
+namespace {
+
+int fail(int status, const char *fmt, ...) {
+    char message[512];
+    va_list args;
+    va_start(args, fmt);
+    vsnprintf(message, sizeof(message), fmt, args);
+    va_end(args);
+    return qlin::set_error(status, message);
+}
+
+bool aligned(const void *p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+
+int check_launch(const char *what) {
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return fail(QLIN_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
+    return qlin::set_error(QLIN_OK, "");
+}
+
+// The byte ranges [a, a + an) and [b, b + bn) share a byte.
+bool overlap(const void *a, size_t an, const void *b, size_t bn) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return x < y + bn && y < x + an;
+}
+
+// Most ids of one grouping (index arithmetic past the last run stays in int).
+constexpr int kMaxIds = 1 << 30;
+
+int check_grouping(const char *what, const int *ids, long count, int groups, const int *order,
+                   const int *slots, const int *offsets, const void *workspace, size_t bytes) {
+    if (count < 1 || count > kMaxIds)
+        return fail(QLIN_ERR_INVALID, "%s: %ld ids (1 to %d)", what, count, kMaxIds);
+    if (groups < 1 || groups > qlin::kMaxGroups)
+        return fail(QLIN_ERR_INVALID, "%s: %d groups (1 to %d)", what, groups, qlin::kMaxGroups);
+    if (!ids || !order || !slots || !offsets)
+        return fail(QLIN_ERR_INVALID, "%s: null pointer", what);
+    if (!aligned(ids, 4) || !aligned(order, 4) || !aligned(slots, 4) || !aligned(offsets, 4))
+        return fail(QLIN_ERR_ALIGNMENT, "%s: index arrays must be 4-byte aligned", what);
+    const size_t need = qlin::group_workspace_bytes(int(count), groups);
+    if (need && (!workspace || bytes < need))
+        return fail(QLIN_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", what, need,
+                    workspace ? bytes : size_t(0));
+    if (need && !aligned(workspace, 4))
+        return fail(QLIN_ERR_ALIGNMENT, "%s: workspace must be 4-byte aligned", what);
+    return QLIN_OK;
+}
+
+// The macro tile for `slots` rows in `experts` groups.
+int choose_tile(long slots, int experts, int N, int K, int fmt, int group) {
+    (void)N;
+    (void)K;
+    (void)fmt;
+    const long each = slots / experts;  // rows per expert, if they are even
+    if (each <= 16) return 1;
+    if (each <= 48) return 4;
+    if (group || each <= 192) return 5;
+    return 7;
+}
+
+int tile_index(const qlin_path &p) {
+    int i = 0;
+    for (const auto &t : qlin::kExpertTiles) {
+        if (t.channels == p.channels && t.tokens == p.tokens && t.waves == p.waves &&
+            (p.kind == QLIN_KIND_SKINNY) == (t.slices > 1))
+            return i;
+        ++i;
+    }
+    return -1;
+}
+
+int check_expert_shape(int slots, int experts, int N, int K, int fmt, int group) {
+    if (fmt != QLIN_I8 && fmt != QLIN_FP8)
+        return fail(QLIN_ERR_INVALID, "unsupported quantized storage type");
+    if (slots < 1 || slots > kMaxIds || N < 1 || K < 1 || K % 16 || N % 16)
+        return fail(QLIN_ERR_INVALID, "grouped GEMM unsupported shape slots=%d N=%d K=%d", slots, N, K);
+    if (experts < 1 || experts > qlin::kMaxGroups)
+        return fail(QLIN_ERR_INVALID, "grouped GEMM: %d experts (1 to %d)", experts, qlin::kMaxGroups);
+    if (fmt == QLIN_I8 && K > INT32_MAX / (128 * 128))
+        return fail(QLIN_ERR_INVALID, "INT8 reduction can overflow INT32");
+    if (group != 0 && group != 128)
+        return fail(QLIN_ERR_INVALID, "grouped GEMM scales are per channel (0) or per 128 of K (got %d)",
+                    group);
+    return QLIN_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t qlin_group_rows_workspace_bytes(int count, int groups) {
+    if (count < 1 || count > kMaxIds || groups < 1 || groups > qlin::kMaxGroups) return 0;
+    return qlin::group_workspace_bytes(count, groups);
+}
+
+int qlin_group_rows(const int *ids, int count, int groups, int *order, int *slots, int *offsets,
+                    void *workspace, size_t workspace_bytes, qlin_stream_t stream) {
+    const int status = check_grouping("group_rows", ids, count, groups, order, slots, offsets,
+                                      workspace, workspace_bytes);
+    if (status) return status;
+    qlin::launch_group_rows({ids, count, groups, order, slots, offsets, workspace},
+                            reinterpret_cast<hipStream_t>(stream));
+    return check_launch("group_rows launch");
+}
+
+int qlin_route(const void *logits, int ld, int logits_type, int tokens, int experts, int top_k,
+               int normalize, int *ids, float *weights, int *order, int *slots, int *offsets,
+               void *workspace, size_t workspace_bytes, qlin_stream_t stream) {
+    if (logits_type != QLIN_F32 && logits_type != QLIN_BF16 && logits_type != QLIN_F16)
+        return fail(QLIN_ERR_INVALID, "router logits must be F32, BF16 or F16");
+    if (tokens < 1 || experts < 1 || experts > qlin::kMaxGroups || ld < experts)
+        return fail(QLIN_ERR_INVALID, "router shape tokens=%d experts=%d ld=%d (1 to %d experts)",
+                    tokens, experts, ld, qlin::kMaxGroups);
+    if (top_k < 1 || top_k > qlin::kMaxTopK || top_k > experts)
+        return fail(QLIN_ERR_INVALID, "router top_k=%d of %d experts (1 to %d)", top_k, experts,
+                    qlin::kMaxTopK);
+    if (!logits || !weights) return fail(QLIN_ERR_INVALID, "router: null pointer");
+    if (!aligned(logits, logits_type == QLIN_F32 ? 4 : 2) || !aligned(weights, 4))
+        return fail(QLIN_ERR_ALIGNMENT, "router logits and weights must be aligned to their type");
+    const int status = check_grouping("router", ids, long(tokens) * top_k, experts, order, slots,
+                                      offsets, workspace, workspace_bytes);
+    if (status) return status;
+    qlin::launch_route({logits, ld, logits_type, tokens, experts, top_k, normalize != 0, ids, weights},
+                       {ids, tokens * top_k, experts, order, slots, offsets, workspace},
+                       reinterpret_cast<hipStream_t>(stream));
+    return check_launch("router launch");
+}
+
+int qlin_combine(const void *h, int h_rows, const int *slots, const float *weights,
+                 const void *base, void *out, int tokens, int top_k, int N, int type,
+                 qlin_stream_t stream) {
+    if (type != QLIN_BF16 && type != QLIN_F16)
+        return fail(QLIN_ERR_INVALID, "combine type must be BF16 or F16");
+    if (h_rows < 1 || tokens < 1 || top_k < 1 || top_k > qlin::kMaxTopK || N < 1)
+        return fail(QLIN_ERR_INVALID, "combine shape h_rows=%d tokens=%d top_k=%d N=%d", h_rows,
+                    tokens, top_k, N);
+    if (long(tokens) * ((long(N) + 2047) / 2048) > INT32_MAX)
+        return fail(QLIN_ERR_INVALID, "combine grid exceeds capacity");
+    if (!h || !slots || !out) return fail(QLIN_ERR_INVALID, "combine: null pointer");
+    if (!aligned(h, 2) || !aligned(base, 2) || !aligned(out, 2) || !aligned(slots, 4) ||
+        !aligned(weights, 4))
+        return fail(QLIN_ERR_ALIGNMENT, "combine operands must be aligned to their type");
+    if (overlap(h, size_t(h_rows) * N * 2, out, size_t(tokens) * N * 2))
+        return fail(QLIN_ERR_INVALID, "combine output overlaps its input rows");
+    if (base && base != out && overlap(base, size_t(tokens) * N * 2, out, size_t(tokens) * N * 2))
+        return fail(QLIN_ERR_INVALID, "combine output overlaps part of its base");
+    qlin::launch_combine({h, slots, weights, base, out, h_rows, tokens, top_k, N, type},
+                         reinterpret_cast<hipStream_t>(stream));
+    return check_launch("combine launch");
+}
+
+int qlin_expert_plan(int slots, int experts, int N, int K, int fmt, int group, qlin_path *path) {
+    if (!path) return fail(QLIN_ERR_INVALID, "path is null");
+    const int status = check_expert_shape(slots, experts, N, K, fmt, group);
+    if (status) return status;
+    const auto &t = qlin::kExpertTiles[choose_tile(slots, experts, N, K, fmt, group)];
+    *path = {t.slices > 1 ? QLIN_KIND_SKINNY : QLIN_KIND_TILED, t.tokens, t.channels, 1, t.waves, 0};
+    return qlin::set_error(QLIN_OK, "");
+}
+
+int qlin_expert_gemm(const qlin_path *path, const void *x, const float *sx, int x_rows,
+                     const int *order, int divisor, const int *offsets, const void *w,
+                     const float *sw, int experts, void *y, int scatter, int slots, int N, int K,
+                     int fmt, int out_type, int group, qlin_stream_t stream) {
+    int status = check_expert_shape(slots, experts, N, K, fmt, group);
+    if (status) return status;
+    if (out_type != QLIN_BF16 && out_type != QLIN_F16)
+        return fail(QLIN_ERR_INVALID, "grouped GEMM output must be F16 or BF16");
+    if (!x || !sx || !offsets || !w || !sw || !y)
+        return fail(QLIN_ERR_INVALID, "grouped GEMM operand pointer is null");
+    if (divisor < 1) return fail(QLIN_ERR_INVALID, "grouped GEMM divisor must be at least 1");
+    if (scatter && !order) return fail(QLIN_ERR_INVALID, "scattered results need the rows' order");
+    if (x_rows < 1 || (!order && x_rows < slots))
+        return fail(QLIN_ERR_INVALID, "grouped GEMM: %d input rows for %d slots", x_rows, slots);
+    if (!aligned(x, 16) || !aligned(w, 16))
+        return fail(QLIN_ERR_ALIGNMENT, "quantized operands must be 16-byte aligned");
+    if (!aligned(y, 8)) return fail(QLIN_ERR_ALIGNMENT, "output must be 8-byte aligned");
+    if (!aligned(sx, 4) || !aligned(sw, group ? 16 : 4))
+        return fail(QLIN_ERR_ALIGNMENT, "scales must be 4-byte aligned (group weight scales 16-byte)");
+    if (!aligned(offsets, 4) || !aligned(order, 4))
+        return fail(QLIN_ERR_ALIGNMENT, "index arrays must be 4-byte aligned");
+    // Gathered rows are addressed through one 32-bit buffer range, and so are a
+    // tile's rows of either operand.
+    if (order && long(x_rows) * K > INT32_MAX)
+        return fail(QLIN_ERR_UNSUPPORTED, "gathered input rows exceed 2 GiB");
+    int tile = choose_tile(slots, experts, N, K, fmt, group);
+    if (path && path->kind) {
+        tile = path->splits == 1 && path->staged == 0 ? tile_index(*path) : -1;
+        if (tile < 0)
+            return fail(QLIN_ERR_UNSUPPORTED, "no grouped %dx%d path of %d waves (kind %d)",
+                        path->channels, path->tokens, path->waves, path->kind);
+    }
+    const auto &t = qlin::kExpertTiles[tile];
+    if (long(t.channels > t.tokens ? t.channels : t.tokens) * K > INT32_MAX)
+        return fail(QLIN_ERR_UNSUPPORTED, "grouped GEMM tile rows exceed 2 GiB");
+    if (qlin::expert_row_tiles(slots, experts, t.tokens) * ((long(N) + t.channels - 1) / t.channels) >
+        INT32_MAX)
+        return fail(QLIN_ERR_UNSUPPORTED, "grouped GEMM has more than 2^31 - 1 macro tiles");
+    qlin::ExpertArgs a{static_cast<const uint8_t *>(x), sx, order, offsets,
+                       static_cast<const uint8_t *>(w), sw, y, x_rows, divisor, scatter != 0,
+                       experts, slots, N, K, fmt, out_type, group};
+    const int r = qlin::launch_expert(a, tile, reinterpret_cast<hipStream_t>(stream));
+    if (r) return fail(r, "no kernel variant for this path");
+    return check_launch("grouped GEMM launch");
+}
+
+size_t qlin_adapter_workspace_bytes(int rows, int adapters, int N, int K, int rank) {
+    if (rows < 1 || adapters < 1 || N < 1 || K < 1 || rank < 1) return 0;
+    return qlin::adapter_workspace_bytes(rows, adapters, N, K, rank);
+}
+
+int qlin_adapter_add(const void *x, int ldx, const int *order, const int *offsets, int rows,
+                     int adapters, const void *a, const void *b, int rank, const int *ranks,
+                     const float *scales, const void *base, void *y, int ldy, int N, int K, int type,
+                     void *workspace, size_t workspace_bytes, qlin_stream_t stream) {
+    if (type != QLIN_BF16 && type != QLIN_F16)
+        return fail(QLIN_ERR_INVALID, "adapter type must be BF16 or F16");
+    if (rows < 1 || rows > kMaxIds || N < 1 || K < 1 || K % 16 || N % 16 || ldx < K || ldy < N)
+        return fail(QLIN_ERR_INVALID, "adapter shape rows=%d N=%d K=%d ldx=%d ldy=%d", rows, N, K,
+                    ldx, ldy);
+    if (adapters < 1 || adapters > qlin::kMaxGroups)
+        return fail(QLIN_ERR_INVALID, "%d adapters (1 to %d)", adapters, qlin::kMaxGroups);
+    if (rank < 1 || rank > 128)
+        return fail(QLIN_ERR_UNSUPPORTED, "adapter rank %d (1 to 128)", rank);
+    if (!x || !order || !offsets || !a || !b || !y)
+        return fail(QLIN_ERR_INVALID, "adapter operand pointer is null");
+    if (!aligned(a, 16) || !aligned(b, 16))
+        return fail(QLIN_ERR_ALIGNMENT, "adapter matrices must be 16-byte aligned");
+    if (!aligned(x, 2) || !aligned(base, 2) || !aligned(y, 2))
+        return fail(QLIN_ERR_ALIGNMENT, "16-bit rows must be 2-byte aligned");
+    if (!aligned(order, 4) || !aligned(offsets, 4) || !aligned(ranks, 4) || !aligned(scales, 4))
+        return fail(QLIN_ERR_ALIGNMENT, "index arrays and scales must be 4-byte aligned");
+    const size_t x_bytes = (size_t(rows - 1) * ldx + K) * 2, y_bytes = (size_t(rows - 1) * ldy + N) * 2;
+    if (overlap(x, x_bytes, y, y_bytes))
+        return fail(QLIN_ERR_INVALID, "adapter output overlaps its input");
+    if (base && base != y && overlap(base, y_bytes, y, y_bytes))
+        return fail(QLIN_ERR_INVALID, "adapter output overlaps part of its base");
+    const size_t need = qlin::adapter_workspace_bytes(rows, adapters, N, K, rank);
+    if (need && (!workspace || workspace_bytes < need))
+        return fail(QLIN_ERR_WORKSPACE, "adapter workspace of %zu bytes needed, %zu given", need,
+                    workspace ? workspace_bytes : size_t(0));
+    if (need && !aligned(workspace, 16))
+        return fail(QLIN_ERR_ALIGNMENT, "workspace must be 16-byte aligned");
+    qlin::launch_adapter({x, order, offsets, a, b, ranks, scales, base, y, ldx, ldy, rows, adapters,
+                          rank, N, K, type, workspace},
+                         reinterpret_cast<hipStream_t>(stream));
+    return check_launch("adapter launch");
+}
+
+}  // extern "C"

@@ -1,0 +1,348 @@
+// Quantized products of rows grouped by expert (qlin_expert_gemm) for gfx950:
+// y[s, :] = D(dequant(x[r(s)] . w[e(s)]^T)) for the slots s of each expert e's
+// range of `offsets`; r(s) = order ? order[s] / divisor : s, the result row s or
+// (scatter) order[s]. INT8 (exact int32) or FP8 codes, per-channel scales
+// ((acc * sx) * sw) or K groups of 128 (fma(p_g, sx_g * sw_g, r), ascending g).
+//
+// The groups' sizes are known on the device only: the grid is the host's
+// upper bound on macro tiles and each workgroup finds its tile (find_tile).
+//
+// Structure: KS slices of K times WN x WM waves. Each slice has an LDS ring of S
+// stages (BN weight rows and BM token rows of 128 K bytes) filled by
+// buffer_load ... lds; the token rows are gathered there, a lane's row offset
+// held in a register for the whole walk. Rows past the group and chunks past K
+// arrive as zeros (out-of-range offsets). The partial tiles of the slices are
+// summed through LDS in ascending slice order.
+#include "qlin_device.hpp"
+#include "qlin_internal.hpp"
+#include "row_groups.hpp"
+
+#include <algorithm>
+#include <type_traits>
+
+namespace qlin {
+#ifdef QLIN_EXPERT_PART
+namespace {
+
+constexpr int kRing = int(kLdsBytes);
+
+template <int Fmt, bool Grouped, int KS, int WN, int WM, int NF, int MT, int S, int EU>
+__global__ __launch_bounds__(64 * KS * WN * WM, EU) void expert_gemm(ExpertArgs p, int tiles_n,
+                                                                     int steps) {
+    using Mma = TileMma<Fmt>;
+    using Acc = typename Mma::Acc;
+    constexpr int NWS = WN * WM, W = KS * NWS;
+    constexpr int BN = 16 * NF * WN, BM = 16 * MT * WM, BK = 128;
+    constexpr int STAGE = (BN + BM) * BK, WI = BN / 8 / NWS, XI = BM / 8 / NWS, INSTS = WI + XI;
+    static_assert(BN / 8 % NWS == 0 && BM / 8 % NWS == 0, "whole DMA instructions per wave");
+    static_assert(S > 1 && (NWS == 1 || NWS % 2 == 0), "the ring refills behind its readers");
+    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+
+    RowTile tile;
+    if (!find_tile(p.offsets, p.experts, p.slots, BM, tiles_n, blockIdx.x, tile)) return;
+    const int K = p.K, N = p.N, n_base = tile.column * BN, m_base = tile.begin;
+    const uint8_t *w = p.w + size_t(tile.group) * N * K;
+    const int k_groups = (K + 127) / 128;
+    const float *sw = p.sw + size_t(tile.group) * N * (Grouped ? k_groups : 1);
+
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int row16 = lane & 15, quad = lane >> 4;
+    const int ks = wave / NWS, ws = wave % NWS, wn = ws % WN, wm = ws / WN;
+    // The tile's row ml in x, or -1 (past the group, or an order entry outside x).
+    auto source = [&](int ml) {
+        if (ml >= tile.rows) return -1;
+        if (!p.order) return m_base + ml;
+        const int at = p.order[m_base + ml];
+        const int row = int(uint32_t(at) / uint32_t(p.divisor));
+        return at >= 0 && row < p.x_rows ? row : -1;
+    };
+
+    const int k_begin = ks * steps * BK;
+    const int count = NWS > 1 ? steps : max(0, min(steps, (K - k_begin + BK - 1) / BK));
+    const int rows_w = min(BN, N - n_base);
+    const __amdgpu_buffer_rsrc_t rsrc_w = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<uint8_t *>(w + size_t(n_base) * K), 0, rows_w * K, 0x00020000);
+    // Gathered rows: offsets from x (the host holds x_rows * K below 2^31); rows
+    // in slot order: from the tile's first row.
+    const __amdgpu_buffer_rsrc_t rsrc_x = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<uint8_t *>(p.order ? p.x : p.x + size_t(m_base) * K), 0,
+        p.order ? p.x_rows * K : tile.rows * K, 0x00020000);
+    // One DMA instruction fills 8 stage rows of 128 bytes in lane order; row r
+    // keeps 16-byte chunk c at c ^ ((r >> 1) & 7) (fragment reads on distinct
+    // banks), so a lane's source chunk goes by the parity of the instruction's
+    // 8-row group (with a shared ring the same for all the wave's).
+    const int lane_row = lane >> 3;
+    const int chunk0 = (lane & 7) ^ (lane_row >> 1) ^ (NWS > 1 ? 4 * (ws & 1) : 0);
+    const int chunk1 = chunk0 ^ 4;
+    const uint32_t woff0 = uint32_t(lane_row) * uint32_t(K) + uint32_t(chunk0 * 16);
+    const uint32_t woff1 = uint32_t(lane_row) * uint32_t(K) + uint32_t(chunk1 * 16);
+    constexpr uint32_t kOut = 0x80000000u;  // an offset past every buffer: reads as zero
+    uint32_t xoff[XI];
+#pragma unroll
+    for (int i = 0; i < XI; ++i) {
+        const int g = NWS > 1 ? i * NWS + ws : i;
+        const int row = source(g * 8 + lane_row);
+        const int chunk = NWS > 1 || !(i & 1) ? chunk0 : chunk1;
+        xoff[i] = row < 0 ? kOut
+                          : uint32_t(p.order ? row : row - m_base) * uint32_t(K) + uint32_t(chunk * 16);
+    }
+    uint8_t *ring = lds + ks * S * STAGE;
+    uint8_t *dma_base = ring;
+    uint32_t dk = 0;
+    bool in0 = true, in1 = true;
+    auto aim = [&](int st, int slot) {
+        dma_base = ring + slot * STAGE;
+        dk = uint32_t(k_begin + st * BK);
+        in0 = int(dk) + chunk0 * 16 < K, in1 = int(dk) + chunk1 * 16 < K;
+    };
+    auto dma = [&](auto i_) {
+        constexpr int i = decltype(i_)::value;
+        constexpr int j = i < WI ? i : i - WI;
+        const bool odd = NWS == 1 && (j & 1);
+        const bool in = odd ? in1 : in0;
+        const uint32_t x_at = in ? xoff[i < WI ? 0 : j] : kOut;
+        const int g = NWS > 1 ? j * NWS + ws : j;  // 8-row group of the operand
+        lds_ptr_t dst = (lds_ptr_t)(dma_base + ((i < WI ? 0 : BN / 8) + g) * 1024);
+        if constexpr (i < WI)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc_w, dst, 16, in ? (odd ? woff1 : woff0) : kOut,
+                                                     uint32_t(g) * 8u * uint32_t(K) + dk, 0, 0);
+        else
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc_x, dst, 16, x_at, dk, 0, 0);
+    };
+    // Wait for a stage with at most `newer` later ones outstanding.
+    auto wait_stage = [&](int newer) {
+        if (newer >= S - 1) wait_vmcnt<INSTS * (S - 1)>();
+        else if (newer == S - 2) wait_vmcnt<INSTS * (S - 2)>();
+        else if (S > 3 && newer == S - 3) wait_vmcnt<INSTS * (S > 3 ? S - 3 : 0)>();
+        else wait_vmcnt<0>();
+    };
+
+    // K groups: the scales of a stage's group, two sets so that the next
+    // stage's arrive under this one's products.
+    struct Scales {
+        f32x4 w[Grouped ? NF : 1];
+        float x[Grouped ? MT : 1];
+    };
+    int sx_row[Grouped ? MT : 1];
+    if constexpr (Grouped) {
+#pragma unroll
+        for (int t = 0; t < MT; ++t) sx_row[t] = max(source((wm * MT + t) * 16 + row16), 0);
+    }
+    auto load_scales = [&](int st, Scales &s) {
+        if constexpr (Grouped) {
+            const int g = min(k_begin / BK + st, k_groups - 1);
+#pragma unroll
+            for (int f = 0; f < NF; ++f) {
+                const int n = min(n_base + (wn * NF + f) * 16 + quad * 4, N - 4);
+                s.w[f] = *reinterpret_cast<const f32x4 *>(sw + size_t(g) * N + n);
+            }
+#pragma unroll
+            for (int t = 0; t < MT; ++t) s.x[t] = p.sx[size_t(g) * p.x_rows + sx_row[t]];
+            if constexpr (KS > 1 && NWS > 1) {
+                // A slice's stages past K add zeros, whatever the last group's scales are.
+                const bool live = k_begin / BK + st < k_groups;
+#pragma unroll
+                for (int f = 0; f < NF; ++f)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) s.w[f][r] = live ? s.w[f][r] : 0.f;
+#pragma unroll
+                for (int t = 0; t < MT; ++t) s.x[t] = live ? s.x[t] : 0.f;
+            }
+        }
+    };
+
+    using Sum = std::conditional_t<Grouped, f32x4, Acc>;
+    Sum acc[NF][MT];
+#pragma unroll
+    for (int f = 0; f < NF; ++f)
+#pragma unroll
+        for (int t = 0; t < MT; ++t) acc[f][t] = Sum{0, 0, 0, 0};
+
+    const int sw7 = (row16 >> 1) & 7;
+    const int c0 = (quad ^ sw7) * 16, c1 = ((4 + quad) ^ sw7) * 16;
+    auto read = [&](int slot, i32x8 (&a)[NF], i32x8 (&b)[MT]) {
+        const uint8_t *q = ring + slot * STAGE + row16 * BK;
+        auto frag = [&](const uint8_t *r) {
+            const i32x4 lo = *reinterpret_cast<const i32x4 *>(r + c0);
+            const i32x4 hi = *reinterpret_cast<const i32x4 *>(r + c1);
+            return i32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+        };
+#pragma unroll
+        for (int t = 0; t < MT; ++t) b[t] = frag(q + (BN + (wm * MT + t) * 16) * BK);
+#pragma unroll
+        for (int f = 0; f < NF; ++f) a[f] = frag(q + (wn * NF + f) * 16 * BK);
+    };
+    // A stage's MFMAs, one (weight, token) tile at a time, with the next DMA's
+    // instructions spread between them.
+    auto mma = [&](auto dma_, const i32x8 (&a)[NF], const i32x8 (&b)[MT], const Scales &s) {
+        constexpr bool kDma = decltype(dma_)::value;
+        static_for<0, NF * MT>([&](auto j_) {
+            constexpr int j = decltype(j_)::value, f = j / MT, t = j % MT;
+            if constexpr (Grouped) {
+                Acc part = Acc{0, 0, 0, 0};
+                Mma::run(part, a[f], b[t]);
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    acc[f][t][r] = __builtin_fmaf(float(part[r]), s.x[t] * s.w[f][r], acc[f][t][r]);
+            } else {
+                Mma::run(acc[f][t], a[f], b[t]);
+            }
+            if constexpr (kDma) {
+                static_for<j * INSTS / (NF * MT), (j + 1) * INSTS / (NF * MT)>(dma);
+                if constexpr (!Grouped) __builtin_amdgcn_sched_barrier(0);
+            }
+        });
+    };
+    Scales s0, s1;
+    load_scales(0, s0);
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int s = 0; s < S; ++s)
+        if (s < count) {
+            aim(s, s);
+            static_for<0, INSTS>(dma);
+        }
+    int slot = 0;  // of the stage whose fragments are in registers
+    // Step s: stage s's fragments have arrived, so its slot is free for stage
+    // s + S (a shared ring: once every wave of the slice has them, after the
+    // barrier, which also makes stage s + 1 visible). Where the ring is deeper
+    // than two or shared, the next fragments are read under this stage's
+    // MFMAs; a private two-stage ring reads them after, giving stage s + 1's
+    // DMA that time to land.
+    auto step = [&](int s, const i32x8 (&a)[NF], const i32x8 (&b)[MT], const Scales &sc,
+                    i32x8 (&na)[NF], i32x8 (&nb)[MT], Scales &nsc) {
+        wait_lds_reads();
+        __builtin_amdgcn_sched_barrier(0);
+        const int next = slot + 1 == S ? 0 : slot + 1;
+        if constexpr (S >= 3 || NWS > 1) {
+            if (s + 1 < count) wait_stage(min(count - 2 - s, S - 2));
+            if constexpr (NWS > 1) __builtin_amdgcn_s_barrier();
+            __builtin_amdgcn_sched_barrier(0);
+            read(next, na, nb);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        load_scales(s + 1, nsc);
+        if (s + S < count) {
+            aim(s + S, slot);
+            mma(std::true_type{}, a, b, sc);
+        } else {
+            mma(std::false_type{}, a, b, sc);
+        }
+        slot = next;
+        if constexpr (S == 2 && NWS == 1) {
+            if (s + 1 < count) wait_stage(count - 2 - s);
+            __builtin_amdgcn_sched_barrier(0);
+            read(slot, na, nb);
+        }
+    };
+    i32x8 a0[NF], b0[MT], a1[NF], b1[MT];
+    if (count > 0) {
+        wait_stage(count - 1);
+        if constexpr (NWS > 1) __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+        read(0, a0, b0);
+        int s = 0;
+        for (; s + 1 < count; s += 2) {
+            step(s, a0, b0, s0, a1, b1, s1);
+            step(s + 1, a1, b1, s1, a0, b0, s0);
+        }
+        if (s < count) step(s, a0, b0, s0, a1, b1, s1);
+    }
+
+    // Sum the slices' partial tiles through LDS (all DMA has landed and been
+    // read), ascending slices; then scales and 8-byte stores, consecutive
+    // threads on consecutive channels.
+    constexpr int PITCH = BN + 4;  // 32-bit values per row of a partial tile
+    static_assert(KS * BM * PITCH * 4 <= kRing, "the slices' partial tiles fit the LDS");
+    constexpr int kRows = 64 * W / (BN / 4), kMaxU = (BM + kRows - 1) / kRows;
+    using Red = std::conditional_t<Fmt == I8 && !Grouped, int, float>;
+    typedef Red Red4 __attribute__((ext_vector_type(4)));
+    Red *red = reinterpret_cast<Red *>(lds);
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int f = 0; f < NF; ++f)
+            *reinterpret_cast<Red4 *>(red + (ks * BM + (wm * MT + t) * 16 + row16) * PITCH +
+                                      (wn * NF + f) * 16 + quad * 4) = acc[f][t];
+    __syncthreads();
+    const int nl = tid % (BN / 4) * 4, r0 = tid / (BN / 4), n = n_base + nl;
+    if (n >= N || r0 >= kRows) return;
+    float scale_w[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) scale_w[r] = Grouped ? 1.f : sw[n + r];
+    for (int u = 0; u < kMaxU; ++u) {
+        const int ml = r0 + u * kRows;
+        if (ml >= tile.rows) break;
+        const int from = source(ml);
+        int to = m_base + ml;
+        if (p.scatter) {
+            to = p.order[to];
+            if (uint32_t(to) >= uint32_t(p.slots)) continue;
+        }
+        Red4 sum = {0, 0, 0, 0};
+#pragma unroll
+        for (int q = 0; q < KS; ++q)
+            sum += *reinterpret_cast<const Red4 *>(red + (q * BM + ml) * PITCH + nl);
+        float v[4];
+        const float scale_x = Grouped ? 1.f : p.sx[max(from, 0)];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const float s = float(sum[r]) * scale_x;
+            v[r] = s * scale_w[r];
+        }
+        uint2 out;
+        if (p.out_type == F16) {
+            out.x = pack2(v[0], v[1], f16_t{});
+            out.y = pack2(v[2], v[3], f16_t{});
+        } else {
+            out.x = pack2(v[0], v[1], bf16_t{});
+            out.y = pack2(v[2], v[3], bf16_t{});
+        }
+        *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p.y) + size_t(to) * N + n) = out;
+    }
+}
+
+template <int Fmt, bool Grouped, int KS, int WN, int WM, int NF, int MT, int S, int EU>
+int launch(const ExpertArgs &a, hipStream_t stream) {
+    constexpr int W = KS * WN * WM, BN = 16 * NF * WN, BM = 16 * MT * WM;
+    constexpr size_t ring = size_t(KS) * S * (BN + BM) * 128;
+    constexpr size_t lds = std::max(ring, size_t(KS) * BM * (BN + 4) * 4);
+    static_assert(lds <= size_t(kRing), "LDS");
+    const int tiles_n = (a.N + BN - 1) / BN;
+    const int steps = ((a.K + 127) / 128 + KS - 1) / KS;
+    hipLaunchKernelGGL((expert_gemm<Fmt, Grouped, KS, WN, WM, NF, MT, S, EU>),
+                       dim3(unsigned(expert_row_tiles(a.slots, a.experts, BM) * tiles_n)),
+                       dim3(64 * W), lds, stream, a, tiles_n, steps);
+    return 0;
+}
+
+template <int Fmt, bool Grouped> int launch_any(const ExpertArgs &a, int tile, hipStream_t s) {
+    switch (tile) {
+#define QLIN_EXPERT_TILE(I, KS, WN, WM, NF, MT, S, EU) \
+    case I: return launch<Fmt, Grouped, KS, WN, WM, NF, MT, S, EU>(a, s);
+        QLIN_EXPERT_TILES(QLIN_EXPERT_TILE)
+#undef QLIN_EXPERT_TILE
+    }
+    return -4;
+}
+
+}  // namespace
+
+int QLIN_EXPERT_PART(const ExpertArgs &a, int tile, hipStream_t s) {
+    return launch_any<QLIN_EXPERT_FMT, QLIN_EXPERT_GROUPED>(a, tile, s);
+}
+#else
+int launch_expert_i8(const ExpertArgs &, int, hipStream_t);
+int launch_expert_i8_grouped(const ExpertArgs &, int, hipStream_t);
+int launch_expert_fp8(const ExpertArgs &, int, hipStream_t);
+int launch_expert_fp8_grouped(const ExpertArgs &, int, hipStream_t);
+int launch_expert(const ExpertArgs &a, int tile, hipStream_t s) {
+    if (a.fmt == I8) return a.group ? launch_expert_i8_grouped(a, tile, s) : launch_expert_i8(a, tile, s);
+    return a.group ? launch_expert_fp8_grouped(a, tile, s) : launch_expert_fp8(a, tile, s);
+}
+#endif
+
+}  // namespace qlin

@@ -147,6 +147,88 @@ constexpr struct { int channels, tokens; } kSlicedTiles[] = {
 size_t packed_weight_bytes(int N, int K);
 void launch_pack_weights(const void *w, int N, int K, void *packed, hipStream_t);
 size_t tiled_workspace_bytes(const GemmArgs &, const GemmPath &);
+// Rows grouped by the weights they use (row_groups.hip).
+constexpr int kMaxGroups = 1024;
+constexpr int kMaxTopK = 16;
+struct RouteArgs {
+    const void *logits;  // [tokens, ld] bf16 / f16 / f32
+    int ld, type, tokens, experts, top_k, normalize;
+    int *ids;            // [tokens, top_k]
+    float *weights;      // [tokens, top_k]
+};
+struct GroupArgs {
+    const int *ids;      // [count]
+    int count, groups;
+    int *order, *slots, *offsets;
+    void *workspace;     // group_workspace_bytes
+};
+size_t group_workspace_bytes(int count, int groups);
+void launch_group_rows(const GroupArgs &, hipStream_t);
+// The router's choices and their grouping (g.ids is r.ids).
+void launch_route(const RouteArgs &, const GroupArgs &, hipStream_t);
+struct CombineArgs {
+    const void *h;         // [h_rows, N] 16-bit
+    const int *slots;      // [tokens, top_k]
+    const float *weights;  // [tokens, top_k] or null (1)
+    const void *base;      // [tokens, N] or null
+    void *out;             // [tokens, N]
+    int h_rows, tokens, top_k, N, type;
+};
+void launch_combine(const CombineArgs &, hipStream_t);
+
+// Products grouped by expert (gemm_experts.hip).
+struct ExpertArgs {
+    const uint8_t *x;    // [x_rows, K]
+    const float *sx;     // [x_rows] or [ceil(K/128), x_rows]
+    const int *order;    // [slots] or null
+    const int *offsets;  // [experts + 1]
+    const uint8_t *w;    // [experts, N, K]
+    const float *sw;     // [experts, N] or [experts, ceil(K/128), N]
+    void *y;             // [slots, N] bf16/f16
+    int x_rows, divisor, scatter, experts, slots, N, K, fmt, out_type, group;
+};
+// Macro tiles: index, K slices, waves along channels and tokens, 16-row
+// fragments per wave of both, LDS stages, waves per SIMD.
+#define QLIN_EXPERT_TILES(X)  \
+    X(0, 8, 1, 1, 1, 1, 4, 2) \
+    X(1, 8, 1, 1, 2, 1, 3, 2) \
+    X(2, 4, 1, 1, 2, 1, 3, 2) \
+    X(3, 4, 1, 1, 4, 1, 3, 1) \
+    X(4, 4, 1, 1, 2, 2, 4, 1) \
+    X(5, 2, 2, 2, 2, 2, 2, 4) \
+    X(6, 1, 2, 4, 4, 2, 4, 2) \
+    X(7, 1, 4, 2, 4, 4, 3, 2) \
+    X(8, 1, 2, 2, 2, 2, 2, 4)
+struct ExpertTile {
+    int channels, tokens, waves, slices;
+};
+#define QLIN_EXPERT_TILE(I, KS, WN, WM, NF, MT, S, EU) \
+    ExpertTile{16 * (NF) * (WN), 16 * (MT) * (WM), (KS) * (WN) * (WM), KS},
+constexpr ExpertTile kExpertTiles[] = {QLIN_EXPERT_TILES(QLIN_EXPERT_TILE)};
+#undef QLIN_EXPERT_TILE
+// Most row tiles that `slots` rows in `groups` groups can make.
+constexpr long expert_row_tiles(long slots, long groups, long height) {
+    return (slots - (slots < groups ? slots : groups)) / height + (slots < groups ? slots : groups);
+}
+int launch_expert(const ExpertArgs &, int tile, hipStream_t);
+
+// Low-rank adapters (adapters.hip).
+struct AdapterArgs {
+    const void *x;       // [rows, ldx] 16-bit
+    const int *order;    // [rows]
+    const int *offsets;  // [adapters + 1]
+    const void *a;       // [adapters, rank, K]
+    const void *b;       // [adapters, N, rank]
+    const int *ranks;    // [adapters] or null
+    const float *scales; // [adapters] or null
+    const void *base;    // [rows, ldy] or null
+    void *y;             // [rows, ldy]
+    int ldx, ldy, rows, adapters, rank, N, K, type;
+    void *workspace;     // adapter_workspace_bytes
+};
+size_t adapter_workspace_bytes(int rows, int adapters, int N, int K, int rank);
+void launch_adapter(const AdapterArgs &, hipStream_t);
+
 // Records `message` as qlin_last_error() of this thread; returns status.
 int set_error(int status, const char *message);
 

@@ -1,0 +1,79 @@
+// Rows grouped by the weights they use: the device side of what
+// qlin_route / qlin_group_rows write and the grouped products read.
+//   offsets [groups + 1]  the slots [offsets[g], offsets[g + 1]) hold group g's rows
+//   order   [slots]       the row (or choice) each slot came from
+// Both live on the device, so a launch is sized by the host's upper bound
+// and each workgroup finds its tile from the offsets.
+#pragma once
+#include "qlin_device.hpp"
+
+namespace qlin {
+namespace {
+
+// Inclusive prefix sum over the 64 lanes: row shifts inside each 16, then the
+// last lane of a 16 / 32 added to the next (lanes without a source add 0).
+__device__ __forceinline__ int wave_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);   // row_shr:1
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);   // row_shr:2
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);   // row_shr:4
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);   // row_shr:8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // row_bcast:15
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // row_bcast:31
+    return v;
+}
+
+// One tile of a grouped product: `rows` slots from `begin` of group `group`,
+// column tile `column`.
+struct RowTile {
+    int group, begin, rows, column;
+};
+
+// The tile of workgroup `index`: the groups' row tiles of at most `height`
+// slots times `columns` column tiles, numbered group by group, each column
+// tile's row tiles in a run (they share the group's weights there), placed
+// XCD-major. False past the last tile. Offsets are held to [0, slots] and
+// ascending order here, so bad ones cannot lead out of the arrays. Same
+// result in every lane of the workgroup.
+__device__ __forceinline__ bool find_tile(const int *__restrict__ offsets, int groups, int slots,
+                                          int height, int columns, int index, RowTile &tile) {
+    const int lane = threadIdx.x & 63;
+    auto load = [&](int g, int &begin) {
+        begin = min(max(offsets[min(g, groups)], 0), slots);
+        const int end = min(offsets[min(g + 1, groups)], slots);
+        return max(end - begin, 0);
+    };
+    int first_begin = 0;
+    const int first_rows = load(lane, first_begin);
+    int mine = (first_rows + height - 1) / height;
+    for (int g = 64 + lane; g < groups; g += 64) {
+        int begin;
+        mine += (load(g, begin) + height - 1) / height;
+    }
+    const int total = __builtin_amdgcn_readlane(wave_scan(mine), 63) * columns;
+    if (index >= total) return false;
+    const int at = xcd_major(index, total);
+    int before = 0;  // row tiles of the groups before this run of 64
+    for (int g0 = 0; g0 < groups; g0 += 64) {
+        int begin = first_begin;
+        const int rows = g0 ? load(g0 + lane, begin) : first_rows;
+        const int tiles = (rows + height - 1) / height;
+        const int upto = before + wave_scan(tiles);
+        const uint64_t past = __ballot(upto * columns > at);
+        if (past) {
+            const int l = __builtin_ctzll(past);
+            const int n = __builtin_amdgcn_readlane(tiles, l);
+            const int in = at - (__builtin_amdgcn_readlane(upto, l) - n) * columns;
+            const int row = in % n * height;
+            tile.group = g0 + l;
+            tile.column = in / n;
+            tile.begin = __builtin_amdgcn_readlane(begin, l) + row;
+            tile.rows = min(height, __builtin_amdgcn_readlane(rows, l) - row);
+            return true;
+        }
+        before = __builtin_amdgcn_readlane(upto, 63);
+    }
+    return false;
+}
+
+}  // namespace
+}  // namespace qlin

@@ -32,6 +32,10 @@
  *                       <- no counterpart in the reference: qlin_linear with its
  *                          scratch in a fixed library-owned device array, for callers
  *                          that cannot allocate
+ *   qlin_route, qlin_group_rows, qlin_combine, qlin_expert_gemm, qlin_expert_plan,
+ *   qlin_adapter_add and their workspace sizes
+ *                       <- no counterpart in the reference: rows that each name the
+ *                          weights they use (experts, codebook heads, adapters)
  *
  * Operand layouts (reference core/quantization.h:24-49):
  *   x  int8/e4m3 [rows, K] dense          sx f32 [rows] or [ceil(K/ig), rows]
@@ -352,6 +356,85 @@ int qlin_linear_noalloc(const qlin_path *path, const void *x, int ld, int src_ty
                         const void *w, const float *sw, void *y, int rows, int N, int K, int fmt,
                         int out_type, int input_group, int weight_group, int rotation,
                         qlin_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * Rows that each name the weights they use: experts of a mixture, heads of a
+ * codebook, adapters of a voice. The rows are grouped once per step on the
+ * device and the products below read the grouping; nothing is copied to the
+ * host, so a step can be captured in a graph and replayed with other rows.
+ *
+ *   ids     [count]       row i's group; outside [0, groups): the row has none
+ *   offsets [groups + 1]  slots [offsets[g], offsets[g + 1]) are group g's rows
+ *   order   [count]       slot -> row, ascending rows in a group; -1 from
+ *                         offsets[groups] on
+ *   slots   [count]       row -> slot, -1 for a row without a group
+ * At most 1024 groups. The consumers hold offsets to [0, slots] in ascending
+ * order and drop entries of order outside their rows. */
+
+/* The grouping of given ids (a stable counting sort; the same bits in every
+ * run). The workspace is needed above 4096 ids. */
+size_t qlin_group_rows_workspace_bytes(int count, int groups);
+int qlin_group_rows(const int *ids, int count, int groups, int *order, int *slots, int *offsets,
+                    void *workspace, size_t workspace_bytes, qlin_stream_t stream);
+
+/* Router: per token the top_k (<= 16) largest of its `experts` logits (row
+ * stride ld; F32, BF16 or F16), ties to the lowest index, in descending order,
+ * and their softmax weights p_j / sum p, p = e^(logit - max), in fp32 (sum over
+ * all experts, or with `normalize` over the chosen); then the grouping of ids
+ * as above with count = tokens * top_k (row t * top_k + j is choice j of token
+ * t). A logit of -inf or NaN is never chosen and weighs nothing; choices that a
+ * token lacks for that reason have id -1 and weight 0. Where the largest is
+ * +inf, the logits at +inf share the weight. Workspace: that of
+ * qlin_group_rows. */
+int qlin_route(const void *logits, int ld, int logits_type, int tokens, int experts, int top_k,
+               int normalize, int *ids, float *weights, int *order, int *slots, int *offsets,
+               void *workspace, size_t workspace_bytes, qlin_stream_t stream);
+
+/* out[t, :] = s16(sum_j weights[t, j] * h[slots[t, j], :] + base[t, :]): the
+ * experts' rows [h_rows, N] back to their tokens, fp32 in ascending j. A slot
+ * outside [0, h_rows) is left out (its row is not read). weights NULL = 1, base
+ * NULL = 0; out may be base. Dense 16-bit rows of one type; top_k <= 16. */
+int qlin_combine(const void *h, int h_rows, const int *slots, const float *weights,
+                 const void *base, void *out, int tokens, int top_k, int N, int type,
+                 qlin_stream_t stream);
+
+/* Quantized product of each group's rows with its own weights:
+ *   y[s, :] = D(dequant(x[r] . w[e]^T)) for the slots s of expert e,
+ *   r = order ? order[s] / divisor : s;  scatter: stored to y[order[s], :].
+ *   x  int8/e4m3 [x_rows, K]      sx f32 [x_rows] or (group 128) [ceil(K/128), x_rows]
+ *   w  int8/e4m3 [experts, N, K]  sw f32 [experts, N] or [experts, ceil(K/128), N]
+ *   y  bf16/f16  [slots, N]       rows of no group are left as they were
+ * `slots` is the capacity of the grouping (the ids' count): offsets say how
+ * many are in use. A router's first product gathers (order, divisor = top_k),
+ * its second reads slots (order NULL); heads or codebooks gather and scatter
+ * (divisor 1). Scaling and shape rules are qlin_gemm's: (acc * sx) * sw, or
+ * fma(p_g, sx_g * sw_g, r) over ascending K groups of each K slice. Gathered
+ * rows must lie in 2 GiB (x_rows * K). `path` may be NULL (planned as
+ * qlin_expert_plan: by slots / experts); its tiles are those that plans of
+ * some shape give. */
+int qlin_expert_plan(int slots, int experts, int N, int K, int fmt, int group, qlin_path *path);
+int qlin_expert_gemm(const qlin_path *path, const void *x, const float *sx, int x_rows,
+                     const int *order, int divisor, const int *offsets, const void *w,
+                     const float *sw, int experts, void *y, int scatter, int slots, int N, int K,
+                     int fmt, int out_type, int group, qlin_stream_t stream);
+
+/* Low-rank adapters of many requests beside a shared projection: for the rows
+ * m of adapter g (order, offsets of qlin_group_rows over the rows' adapters)
+ *   y[m, :] = s16(base[m, :] + scales[g] * (x[m, :] . a[g]^T) . b[g]^T)
+ *   x 16-bit [rows, ldx]   a 16-bit [adapters, rank, K]   b 16-bit [adapters, N, rank]
+ *   base, y 16-bit [rows, ldy] (base NULL = 0; y may be base, the projection's
+ *   output); rows without an adapter are left as they were
+ *   ranks [adapters] or NULL: the ranks in use; the rest of a and b is not used
+ *   scales f32 [adapters] or NULL (1)
+ * Both products accumulate in fp32 and the inner one is carried with 18 bits
+ * or more. rank <= 128, K % 16 == 0, N % 16 == 0; order names a row at most once.
+ * A column range of y (one projection of a merged output) is a y offset by its
+ * first column with the whole row's ldy. */
+size_t qlin_adapter_workspace_bytes(int rows, int adapters, int N, int K, int rank);
+int qlin_adapter_add(const void *x, int ldx, const int *order, const int *offsets, int rows,
+                     int adapters, const void *a, const void *b, int rank, const int *ranks,
+                     const float *scales, const void *base, void *y, int ldy, int N, int K, int type,
+                     void *workspace, size_t workspace_bytes, qlin_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,155 @@
+"""Refusals of the operators on grouped rows, without a GPU: every call below
+fails its checks before anything reaches the device."""
+import ctypes
+
+import pytest
+import torch
+
+from breeze_tts_cpp_amd import qlinear
+
+BF16, F32, I32, FP8, I8, F16 = 0, 1, 2, 3, 4, 5
+FAKE = 0x10000  # never dereferenced
+FAR = 0x40000000000
+
+
+def test_group_rows_refusals():
+    L = qlinear.load()
+
+    def call(ids=FAKE, count=100, groups=8, order=FAKE, slots=FAKE, offsets=FAKE, ws=None, wsb=0):
+        return L.qlin_group_rows(ids, count, groups, order, slots, offsets, ws, wsb, None)
+
+    assert call(count=0) == -1 and call(count=(1 << 30) + 1) == -1
+    assert call(groups=0) == -1 and call(groups=1025) == -1
+    for name in ("ids", "order", "slots", "offsets"):
+        assert call(**{name: None}) == -1
+        assert call(**{name: FAKE + 2}) == -2
+    need = L.qlin_group_rows_workspace_bytes(100000, 8)
+    assert need > 0 and L.qlin_group_rows_workspace_bytes(4096, 1024) == 0
+    assert call(count=100000) == -3 and b"workspace" in L.qlin_last_error()
+    assert call(count=100000, ws=FAKE, wsb=need - 1) == -3
+    assert call(count=100000, ws=FAKE + 2, wsb=need) == -2
+    assert L.qlin_group_rows_workspace_bytes(0, 8) == 0
+    assert L.qlin_group_rows_workspace_bytes(10, 2000) == 0
+
+
+def test_route_refusals():
+    L = qlinear.load()
+
+    def call(logits=FAKE, ld=64, t=F32, tokens=4, experts=64, k=2, ids=FAKE, w=FAKE, order=FAKE,
+             slots=FAKE, off=FAKE, ws=None, wsb=0):
+        return L.qlin_route(logits, ld, t, tokens, experts, k, 0, ids, w, order, slots, off, ws, wsb,
+                            None)
+
+    assert call(t=I8) == -1 and call(tokens=0) == -1 and call(experts=0) == -1
+    assert call(experts=1025, ld=1025) == -1 and call(ld=63) == -1
+    assert call(k=0) == -1 and call(k=17) == -1 and call(experts=3, k=4) == -1
+    for name in ("logits", "ids", "w", "order", "slots", "off"):
+        assert call(**{name: None}) == -1
+    assert call(logits=FAKE + 2) == -2 and call(w=FAKE + 2) == -2
+    assert call(t=BF16, logits=FAKE + 1) == -2
+    assert call(tokens=4096, k=2) == -3
+    assert call(tokens=1 << 29, k=8) == -1  # more choices than an index holds
+
+
+def test_combine_refusals():
+    L = qlinear.load()
+
+    def call(h=FAKE, rows=8, slots=FAKE, w=FAKE, base=None, out=FAR, tokens=4, k=2, N=64, t=BF16):
+        return L.qlin_combine(h, rows, slots, w, base, out, tokens, k, N, t, None)
+
+    assert call(t=F32) == -1 and call(rows=0) == -1 and call(tokens=0) == -1
+    assert call(k=0) == -1 and call(k=17) == -1 and call(N=0) == -1
+    for name in ("h", "slots", "out"):
+        assert call(**{name: None}) == -1
+    assert call(h=FAKE + 1) == -2 and call(slots=FAKE + 2) == -2 and call(w=FAKE + 1) == -2
+    assert call(out=FAKE + 512) == -1                      # inside h
+    assert call(base=FAR + 2, out=FAR) == -1               # shifted base
+    assert call(tokens=1 << 30, N=8192) == -1
+
+
+def test_expert_refusals():
+    L = qlinear.load()
+
+    def call(path=None, x=FAKE, sx=FAKE, x_rows=64, order=FAKE, div=1, off=FAKE, w=FAKE, sw=FAKE,
+             experts=8, y=FAKE, scatter=0, slots=64, N=64, K=256, fmt=I8, out=BF16, group=0):
+        p = ctypes.byref(path.to_c()) if path else None
+        return L.qlin_expert_gemm(p, x, sx, x_rows, order, div, off, w, sw, experts, y, scatter,
+                                  slots, N, K, fmt, out, group, None)
+
+    assert call(fmt=BF16) == -1 and call(out=F32) == -1
+    assert call(K=200) == -1 and call(N=40) == -1 and call(slots=0) == -1 and call(K=131072) == -1
+    assert call(experts=0) == -1 and call(experts=1025) == -1
+    assert call(group=64) == -1
+    for name in ("x", "sx", "off", "w", "sw", "y"):
+        assert call(**{name: None}) == -1
+    assert call(div=0) == -1
+    assert call(order=None, scatter=1) == -1
+    assert call(order=None, x_rows=63) == -1 and call(x_rows=0) == -1
+    assert call(x=FAKE + 8) == -2 and call(w=FAKE + 8) == -2 and call(y=FAKE + 4) == -2
+    assert call(sx=FAKE + 2) == -2 and call(sw=FAKE + 4, group=128) == -2
+    assert call(order=FAKE + 2) == -2
+    assert call(x_rows=1 << 20, K=2048) == -4 and b"2 GiB" in L.qlin_last_error()
+    assert call(path=qlinear.Path(qlinear.KIND_SKINNY, 16, 48, 1, 8)) == -4
+    good = qlinear.expert_plan(64, 8, 64, 256, I8)
+    assert call(path=qlinear.Path(good.kind, good.tokens, good.channels, 2, good.waves)) == -4
+    assert call(path=qlinear.Path(good.kind, good.tokens, good.channels, 1, good.waves + 1)) == -4
+    assert call(slots=1 << 30, order=FAKE, x_rows=1, N=1 << 20, K=16) == -4
+    p = qlinear.qlin_path()
+    assert L.qlin_expert_plan(64, 8, 64, 256, I8, 0, None) == -1
+    assert L.qlin_expert_plan(64, 8, 60, 256, I8, 0, ctypes.byref(p)) == -1
+
+
+def test_adapter_refusals():
+    L = qlinear.load()
+
+    def call(x=FAKE, ldx=256, order=FAKE, off=FAKE, rows=8, n=4, a=FAKE, b=FAKE, rank=16, ranks=None,
+             scales=None, base=None, y=FAR, ldy=64, N=64, K=256, t=BF16, ws=None, wsb=0):
+        return L.qlin_adapter_add(x, ldx, order, off, rows, n, a, b, rank, ranks, scales, base, y,
+                                  ldy, N, K, t, ws, wsb, None)
+
+    assert call(t=F32) == -1 and call(rows=0) == -1 and call(N=40) == -1 and call(K=200) == -1
+    assert call(ldx=255) == -1 and call(ldy=63) == -1
+    assert call(n=0) == -1 and call(n=1025) == -1
+    assert call(rank=0) == -4 and call(rank=129) == -4
+    for name in ("x", "order", "off", "a", "b", "y"):
+        assert call(**{name: None}) == -1
+    assert call(a=FAKE + 8) == -2 and call(b=FAKE + 2) == -2 and call(x=FAKE + 1) == -2
+    assert call(order=FAKE + 2) == -2 and call(scales=FAKE + 1) == -2 and call(ranks=FAKE + 2) == -2
+    assert call(y=FAKE + 64) == -1 and b"overlaps" in L.qlin_last_error()
+    assert call(base=FAR + 2) == -1
+    need = L.qlin_adapter_workspace_bytes(4096, 4, 64, 256, 16)
+    assert need > 0
+    assert call(rows=4096) == -3 and call(rows=4096, ws=FAKE, wsb=need - 1) == -3
+    assert call(rows=4096, ws=FAKE + 4, wsb=need) == -2
+
+
+def test_binding_refusals():
+    """Shapes and types that the Python binding turns away itself."""
+    i32 = torch.int32
+    order, offsets = torch.zeros(4, dtype=i32), torch.zeros(3, dtype=i32)
+    with pytest.raises(ValueError):
+        qlinear.group_rows(torch.zeros(4, dtype=torch.int64), 2)
+    with pytest.raises(ValueError):
+        qlinear.route(torch.zeros(4, 8, dtype=torch.int8), 2)
+    with pytest.raises(ValueError):
+        qlinear.combine(torch.zeros(4, 8), torch.zeros(2, 2, dtype=i32))
+    h = torch.zeros(4, 8, dtype=torch.bfloat16)
+    with pytest.raises(ValueError):
+        qlinear.combine(h, torch.zeros(2, 2, dtype=i32), torch.zeros(2, 3))
+    with pytest.raises(ValueError):
+        qlinear.combine(h, torch.zeros(2, 2, dtype=i32), base=torch.zeros(3, 8, dtype=torch.bfloat16))
+    x, w = torch.zeros(4, 32, dtype=torch.uint8), torch.zeros(2, 16, 32, dtype=torch.uint8)
+    with pytest.raises(ValueError):
+        qlinear.expert_gemm(x, torch.zeros(4), w, torch.zeros(2, 15), I8, offsets)
+    with pytest.raises(ValueError):
+        qlinear.expert_gemm(x, torch.zeros(4), w, torch.zeros(2, 16), I8, offsets[:2])
+    with pytest.raises(ValueError):
+        qlinear.expert_gemm(x[:, :16], torch.zeros(4), w, torch.zeros(2, 16), I8, offsets)
+    xb, a = torch.zeros(4, 32, dtype=torch.bfloat16), torch.zeros(2, 8, 32, dtype=torch.bfloat16)
+    b, y = torch.zeros(2, 16, 8, dtype=torch.bfloat16), torch.zeros(4, 16, dtype=torch.bfloat16)
+    with pytest.raises(ValueError):
+        qlinear.adapter_add(xb, order, offsets, a, b.float(), y)
+    with pytest.raises(ValueError):
+        qlinear.adapter_add(xb, order[:3], offsets, a, b, y)
+    with pytest.raises(ValueError):
+        qlinear.adapter_add(xb, order, offsets, a, b, y, base=torch.zeros(4, 32, dtype=torch.bfloat16)[:, :16])
