@@ -24,7 +24,19 @@ namespace qlin {
 #ifdef QLIN_EXPERT_PART
 namespace {
 
-constexpr int kRing = int(kLdsBytes);
+// LDS of the slices' rings; afterwards of the partial tiles (one slice: of the
+// 16-bit results).
+constexpr int expert_body_bytes(int slices, int stages, int bn, int bm) {
+    const int ring = slices * stages * (bn + bm) * 128;
+    const int sums = slices == 1 ? bm * (bn + 8) * 2 : slices * bm * (bn + 4) * 4;
+    return ring > sums ? ring : sums;
+}
+
+// No memory access or other instruction is moved across.
+__device__ __forceinline__ void pin() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
 
 template <int Fmt, bool Grouped, int KS, int WN, int WM, int NF, int MT, int S, int EU>
 __global__ __launch_bounds__(64 * KS * WN * WM, EU) void expert_gemm(ExpertArgs p, int tiles_n,
@@ -78,15 +90,9 @@ __global__ __launch_bounds__(64 * KS * WN * WM, EU) void expert_gemm(ExpertArgs 
     const uint32_t woff0 = uint32_t(lane_row) * uint32_t(K) + uint32_t(chunk0 * 16);
     const uint32_t woff1 = uint32_t(lane_row) * uint32_t(K) + uint32_t(chunk1 * 16);
     constexpr uint32_t kOut = 0x80000000u;  // an offset past every buffer: reads as zero
-    uint32_t xoff[XI];
+    int xrow[XI];
 #pragma unroll
-    for (int i = 0; i < XI; ++i) {
-        const int g = NWS > 1 ? i * NWS + ws : i;
-        const int row = source(g * 8 + lane_row);
-        const int chunk = NWS > 1 || !(i & 1) ? chunk0 : chunk1;
-        xoff[i] = row < 0 ? kOut
-                          : uint32_t(p.order ? row : row - m_base) * uint32_t(K) + uint32_t(chunk * 16);
-    }
+    for (int i = 0; i < XI; ++i) xrow[i] = source((NWS > 1 ? i * NWS + ws : i) * 8 + lane_row);
     uint8_t *ring = lds + ks * S * STAGE;
     uint8_t *dma_base = ring;
     uint32_t dk = 0;
@@ -96,27 +102,49 @@ __global__ __launch_bounds__(64 * KS * WN * WM, EU) void expert_gemm(ExpertArgs 
         dk = uint32_t(k_begin + st * BK);
         in0 = int(dk) + chunk0 * 16 < K, in1 = int(dk) + chunk1 * 16 < K;
     };
+    auto dma_w = [&](auto j_) {
+        constexpr int j = decltype(j_)::value;
+        const int g = NWS > 1 ? j * NWS + ws : j;  // 8-row group of the operand
+        const bool odd = NWS == 1 && (j & 1);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(
+            rsrc_w, (lds_ptr_t)(dma_base + g * 1024), 16, (odd ? in1 : in0) ? (odd ? woff1 : woff0) : kOut,
+            uint32_t(g) * 8u * uint32_t(K) + dk, 0, 0);
+    };
+    uint32_t xoff[XI];
+    auto dma_x = [&](auto j_) {
+        constexpr int j = decltype(j_)::value;
+        const int g = NWS > 1 ? j * NWS + ws : j;
+        const uint32_t at = (NWS == 1 && (j & 1) ? in1 : in0) ? xoff[j] : kOut;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc_x, (lds_ptr_t)(dma_base + (BN / 8 + g) * 1024), 16, at,
+                                                 dk, 0, 0);
+    };
     auto dma = [&](auto i_) {
         constexpr int i = decltype(i_)::value;
-        constexpr int j = i < WI ? i : i - WI;
-        const bool odd = NWS == 1 && (j & 1);
-        const bool in = odd ? in1 : in0;
-        const uint32_t x_at = in ? xoff[i < WI ? 0 : j] : kOut;
-        const int g = NWS > 1 ? j * NWS + ws : j;  // 8-row group of the operand
-        lds_ptr_t dst = (lds_ptr_t)(dma_base + ((i < WI ? 0 : BN / 8) + g) * 1024);
-        if constexpr (i < WI)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc_w, dst, 16, in ? (odd ? woff1 : woff0) : kOut,
-                                                     uint32_t(g) * 8u * uint32_t(K) + dk, 0, 0);
-        else
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc_x, dst, 16, x_at, dk, 0, 0);
+        if constexpr (i < WI) dma_w(std::integral_constant<int, i < WI ? i : 0>{});
+        else dma_x(std::integral_constant<int, i < WI ? 0 : i - WI>{});
     };
-    // Wait for a stage with at most `newer` later ones outstanding.
-    auto wait_stage = [&](int newer) {
-        if (newer >= S - 1) wait_vmcnt<INSTS * (S - 1)>();
-        else if (newer == S - 2) wait_vmcnt<INSTS * (S - 2)>();
-        else if (S > 3 && newer == S - 3) wait_vmcnt<INSTS * (S > 3 ? S - 3 : 0)>();
-        else wait_vmcnt<0>();
-    };
+
+    // Where all of a slice's stages fit its ring, their weights are asked for
+    // before the rows' addresses are known (those wait for the offsets, then
+    // the order).
+    const bool whole = count <= S;
+    __builtin_amdgcn_sched_barrier(0);
+    if (whole) {
+#pragma unroll
+        for (int s = 0; s < S; ++s)
+            if (s < count) {
+                aim(s, s);
+                static_for<0, WI>(dma_w);
+            }
+        __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int i = 0; i < XI; ++i) {
+        const int chunk = NWS > 1 || !(i & 1) ? chunk0 : chunk1;
+        xoff[i] = xrow[i] < 0 ? kOut
+                              : uint32_t(p.order ? xrow[i] : xrow[i] - m_base) * uint32_t(K) +
+                                    uint32_t(chunk * 16);
+    }
 
     // K groups: the scales of a stage's group, two sets so that the next
     // stage's arrive under this one's products.
@@ -151,6 +179,25 @@ __global__ __launch_bounds__(64 * KS * WN * WM, EU) void expert_gemm(ExpertArgs 
             }
         }
     };
+    Scales s0, s1;
+    load_scales(0, s0);
+
+    // For the epilogue, in LDS past the ring: the rows' scales and where they go, the
+    // channels' scales.
+    constexpr int kBody = expert_body_bytes(KS, S, BN, BM);
+    float *row_scale = reinterpret_cast<float *>(lds + kBody), *col_scale = row_scale + BM;
+    int *row_to = reinterpret_cast<int *>(col_scale + BN);
+    for (int i = tid; i < BM; i += 64 * W) {
+        const int from = source(i);
+        int to = i < tile.rows ? m_base + i : -1;
+        if (p.scatter && to >= 0) {
+            to = p.order[to];
+            if (uint32_t(to) >= uint32_t(p.slots)) to = -1;
+        }
+        row_to[i] = to;
+        row_scale[i] = Grouped ? 1.f : p.sx[max(from, 0)];
+    }
+    for (int i = tid; i < BN; i += 64 * W) col_scale[i] = Grouped ? 1.f : sw[min(n_base + i, N - 1)];
 
     using Sum = std::conditional_t<Grouped, f32x4, Acc>;
     Sum acc[NF][MT];
@@ -161,156 +208,190 @@ __global__ __launch_bounds__(64 * KS * WN * WM, EU) void expert_gemm(ExpertArgs 
 
     const int sw7 = (row16 >> 1) & 7;
     const int c0 = (quad ^ sw7) * 16, c1 = ((4 + quad) ^ sw7) * 16;
-    auto read = [&](int slot, i32x8 (&a)[NF], i32x8 (&b)[MT]) {
-        const uint8_t *q = ring + slot * STAGE + row16 * BK;
-        auto frag = [&](const uint8_t *r) {
-            const i32x4 lo = *reinterpret_cast<const i32x4 *>(r + c0);
-            const i32x4 hi = *reinterpret_cast<const i32x4 *>(r + c1);
-            return i32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-        };
-#pragma unroll
-        for (int t = 0; t < MT; ++t) b[t] = frag(q + (BN + (wm * MT + t) * 16) * BK);
-#pragma unroll
-        for (int f = 0; f < NF; ++f) a[f] = frag(q + (wn * NF + f) * 16 * BK);
+    auto frag = [&](int slot, int row) {
+        const uint8_t *q = ring + slot * STAGE + (row + row16) * BK;
+        const i32x4 lo = *reinterpret_cast<const i32x4 *>(q + c0);
+        const i32x4 hi = *reinterpret_cast<const i32x4 *>(q + c1);
+        return i32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
     };
-    // A stage's MFMAs, one (weight, token) tile at a time, with the next DMA's
-    // instructions spread between them.
-    auto mma = [&](auto dma_, const i32x8 (&a)[NF], const i32x8 (&b)[MT], const Scales &s) {
-        constexpr bool kDma = decltype(dma_)::value;
-        static_for<0, NF * MT>([&](auto j_) {
-            constexpr int j = decltype(j_)::value, f = j / MT, t = j % MT;
+    auto read_x = [&](int slot, i32x8 (&b)[MT]) {
+#pragma unroll
+        for (int t = 0; t < MT; ++t) b[t] = frag(slot, BN + (wm * MT + t) * 16);
+    };
+    auto read_w = [&](int slot, int f) { return frag(slot, (wn * NF + f) * 16); };
+    // Products of weight fragment f with the stage's token fragments.
+    auto row = [&](auto f_, const i32x8 &a, const i32x8 (&b)[MT], const Scales &s) {
+        constexpr int f = decltype(f_)::value;
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
             if constexpr (Grouped) {
                 Acc part = Acc{0, 0, 0, 0};
-                Mma::run(part, a[f], b[t]);
+                Mma::run(part, a, b[t]);
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
                     acc[f][t][r] = __builtin_fmaf(float(part[r]), s.x[t] * s.w[f][r], acc[f][t][r]);
             } else {
-                Mma::run(acc[f][t], a[f], b[t]);
+                Mma::run(acc[f][t], a, b[t]);
             }
-            if constexpr (kDma) {
-                static_for<j * INSTS / (NF * MT), (j + 1) * INSTS / (NF * MT)>(dma);
-                if constexpr (!Grouped) __builtin_amdgcn_sched_barrier(0);
-            }
-        });
+        }
     };
-    Scales s0, s1;
-    load_scales(0, s0);
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_sched_barrier(0);
+
+    // The rest of the first stages' DMA.
+    pin();
 #pragma unroll
     for (int s = 0; s < S; ++s)
         if (s < count) {
             aim(s, s);
-            static_for<0, INSTS>(dma);
+            if (!whole) static_for<0, WI>(dma_w);
+            static_for<0, XI>(dma_x);
         }
-    int slot = 0;  // of the stage whose fragments are in registers
-    // Step s: stage s's fragments have arrived, so its slot is free for stage
-    // s + S (a shared ring: once every wave of the slice has them, after the
-    // barrier, which also makes stage s + 1 visible). Where the ring is deeper
-    // than two or shared, the next fragments are read under this stage's
-    // MFMAs; a private two-stage ring reads them after, giving stage s + 1's
-    // DMA that time to land.
-    auto step = [&](int s, const i32x8 (&a)[NF], const i32x8 (&b)[MT], const Scales &sc,
-                    i32x8 (&na)[NF], i32x8 (&nb)[MT], Scales &nsc) {
-        wait_lds_reads();
-        __builtin_amdgcn_sched_barrier(0);
-        const int next = slot + 1 == S ? 0 : slot + 1;
-        if constexpr (S >= 3 || NWS > 1) {
-            if (s + 1 < count) wait_stage(min(count - 2 - s, S - 2));
-            if constexpr (NWS > 1) __builtin_amdgcn_s_barrier();
-            __builtin_amdgcn_sched_barrier(0);
-            read(next, na, nb);
-            __builtin_amdgcn_sched_barrier(0);
-        }
-        load_scales(s + 1, nsc);
-        if (s + S < count) {
-            aim(s + S, slot);
-            mma(std::true_type{}, a, b, sc);
+    // Wait for stage `st` with `newer` later ones asked for.
+    auto wait_stage = [&](int newer) {
+        if (whole) {
+            if (newer >= 3 && S > 3) wait_vmcnt<XI * 3>();
+            else if (newer == 2) wait_vmcnt<XI * 2>();
+            else if (newer == 1) wait_vmcnt<XI>();
+            else wait_vmcnt<0>();
         } else {
-            mma(std::false_type{}, a, b, sc);
-        }
-        slot = next;
-        if constexpr (S == 2 && NWS == 1) {
-            if (s + 1 < count) wait_stage(count - 2 - s);
-            __builtin_amdgcn_sched_barrier(0);
-            read(slot, na, nb);
+            if (newer >= 3 && S > 3) wait_vmcnt<INSTS * 3>();
+            else if (newer == 2) wait_vmcnt<INSTS * 2>();
+            else if (newer == 1) wait_vmcnt<INSTS>();
+            else wait_vmcnt<0>();
         }
     };
-    i32x8 a0[NF], b0[MT], a1[NF], b1[MT];
-    if (count > 0) {
-        wait_stage(count - 1);
+    static_assert(S <= 4, "the waits above");
+    int slot = 0;  // of the stage whose token fragments are in registers
+    // Step s: at its start every read of stage s - 1 has arrived (with a shared
+    // ring in every wave), so that stage's slot takes stage s - 1 + S. Weight
+    // fragments are read one 16-row block ahead of their MFMAs, the next stage's
+    // token fragments and first weight fragment under the last block's, once
+    // that stage has landed (with a shared ring for every wave: the barrier).
+    auto step = [&](int s, i32x8 &a, const i32x8 (&b)[MT], const Scales &sc, i32x8 (&nb)[MT],
+                    Scales &nsc) {
+        load_scales(s + 1, nsc);
+        if (s > 0 && s - 1 + S < count) {
+            aim(s - 1 + S, slot == 0 ? S - 1 : slot - 1);
+            static_for<0, INSTS>(dma);
+        }
+        static_for<0, NF - 1>([&](auto f_) {
+            const i32x8 an = read_w(slot, decltype(f_)::value + 1);
+            row(f_, a, b, sc);
+            a = an;
+            pin();  // (a stage's weight fragments at once do not fit the registers)
+        });
+        slot = slot + 1 == S ? 0 : slot + 1;
+        if (s + 1 < count) wait_stage(min(s - 1 + S, count - 1) - (s + 1));
+        pin();
+        wait_lds_reads();
         if constexpr (NWS > 1) __builtin_amdgcn_s_barrier();
-        __builtin_amdgcn_sched_barrier(0);
-        read(0, a0, b0);
+        pin();
+        // (After the last stage a slot whose fragments go unused: a conditional
+        // read would copy every fragment.)
+        read_x(slot, nb);
+        const i32x8 an = read_w(slot, 0);
+        row(std::integral_constant<int, NF - 1>{}, a, b, sc);
+        a = an;
+    };
+    i32x8 a, b0[MT], b1[MT];
+    if (count > 0) {
+        wait_stage(min(S, count) - 1);
+        if constexpr (NWS > 1) __builtin_amdgcn_s_barrier();
+        pin();
+        read_x(0, b0);
+        a = read_w(0, 0);
         int s = 0;
         for (; s + 1 < count; s += 2) {
-            step(s, a0, b0, s0, a1, b1, s1);
-            step(s + 1, a1, b1, s1, a0, b0, s0);
+            step(s, a, b0, s0, b1, s1);
+            step(s + 1, a, b1, s1, b0, s0);
         }
-        if (s < count) step(s, a0, b0, s0, a1, b1, s1);
+        if (s < count) step(s, a, b0, s0, b1, s1);
     }
+    wait_lds_reads();
+    __syncthreads();
 
-    // Sum the slices' partial tiles through LDS (all DMA has landed and been
-    // read), ascending slices; then scales and 8-byte stores, consecutive
-    // threads on consecutive channels.
-    constexpr int PITCH = BN + 4;  // 32-bit values per row of a partial tile
-    static_assert(KS * BM * PITCH * 4 <= kRing, "the slices' partial tiles fit the LDS");
-    constexpr int kRows = 64 * W / (BN / 4), kMaxU = (BM + kRows - 1) / kRows;
-    using Red = std::conditional_t<Fmt == I8 && !Grouped, int, float>;
-    typedef Red Red4 __attribute__((ext_vector_type(4)));
-    Red *red = reinterpret_cast<Red *>(lds);
-    __syncthreads();
+    // Scales and stores. One slice: the 16-bit results go through LDS to whole
+    // 16-byte pieces of rows. More: the partial tiles are summed there,
+    // ascending slices.
+    if constexpr (KS == 1) {
+        constexpr int PITCH = BN + 8, kPieces = BN / 8, kPass = 64 * W / kPieces;
+        static_assert(64 * W % kPieces == 0, "whole rows per pass");
+        uint16_t *tile16 = reinterpret_cast<uint16_t *>(lds);
 #pragma unroll
-    for (int t = 0; t < MT; ++t)
+        for (int t = 0; t < MT; ++t) {
+            const int ml = (wm * MT + t) * 16 + row16;
+            const float scale_x = row_scale[ml];
 #pragma unroll
-        for (int f = 0; f < NF; ++f)
-            *reinterpret_cast<Red4 *>(red + (ks * BM + (wm * MT + t) * 16 + row16) * PITCH +
-                                      (wn * NF + f) * 16 + quad * 4) = acc[f][t];
-    __syncthreads();
-    const int nl = tid % (BN / 4) * 4, r0 = tid / (BN / 4), n = n_base + nl;
-    if (n >= N || r0 >= kRows) return;
-    float scale_w[4];
+            for (int f = 0; f < NF; ++f) {
+                const int nl = (wn * NF + f) * 16 + quad * 4;
+                float v[4];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) scale_w[r] = Grouped ? 1.f : sw[n + r];
-    for (int u = 0; u < kMaxU; ++u) {
-        const int ml = r0 + u * kRows;
-        if (ml >= tile.rows) break;
-        const int from = source(ml);
-        int to = m_base + ml;
-        if (p.scatter) {
-            to = p.order[to];
-            if (uint32_t(to) >= uint32_t(p.slots)) continue;
+                for (int r = 0; r < 4; ++r) {
+                    const float s = float(acc[f][t][r]) * scale_x;
+                    v[r] = s * col_scale[nl + r];
+                }
+                *reinterpret_cast<uint2 *>(tile16 + ml * PITCH + nl) =
+                    p.out_type == F16 ? uint2{pack2(v[0], v[1], f16_t{}), pack2(v[2], v[3], f16_t{})}
+                                      : uint2{pack2(v[0], v[1], bf16_t{}), pack2(v[2], v[3], bf16_t{})};
+            }
         }
-        Red4 sum = {0, 0, 0, 0};
-#pragma unroll
-        for (int q = 0; q < KS; ++q)
-            sum += *reinterpret_cast<const Red4 *>(red + (q * BM + ml) * PITCH + nl);
-        float v[4];
-        const float scale_x = Grouped ? 1.f : p.sx[max(from, 0)];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const float s = float(sum[r]) * scale_x;
-            v[r] = s * scale_w[r];
+        __syncthreads();
+        const int nl = tid % kPieces * 8;
+        const bool whole16 = reinterpret_cast<uintptr_t>(p.y) % 16 == 0;
+        if (n_base + nl < N) {
+#pragma unroll 4
+            for (int ml = tid / kPieces; ml < BM; ml += kPass) {
+                const int to = row_to[ml];
+                const uint4 v = *reinterpret_cast<const uint4 *>(tile16 + ml * PITCH + nl);
+                uint16_t *dst = static_cast<uint16_t *>(p.y) + size_t(max(to, 0)) * N + n_base + nl;
+                if (to < 0) continue;
+                if (whole16) {
+                    *reinterpret_cast<uint4 *>(dst) = v;
+                } else {
+                    reinterpret_cast<uint2 *>(dst)[0] = uint2{v.x, v.y};
+                    reinterpret_cast<uint2 *>(dst)[1] = uint2{v.z, v.w};
+                }
+            }
         }
-        uint2 out;
-        if (p.out_type == F16) {
-            out.x = pack2(v[0], v[1], f16_t{});
-            out.y = pack2(v[2], v[3], f16_t{});
-        } else {
-            out.x = pack2(v[0], v[1], bf16_t{});
-            out.y = pack2(v[2], v[3], bf16_t{});
+    } else {
+        constexpr int PITCH = BN + 4;  // 32-bit values per row of a partial tile
+        constexpr int kPass = 64 * W / (BN / 4);
+        using Red = std::conditional_t<Fmt == I8 && !Grouped, int, float>;
+        typedef Red Red4 __attribute__((ext_vector_type(4)));
+        Red *red = reinterpret_cast<Red *>(lds);
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+            for (int f = 0; f < NF; ++f)
+                *reinterpret_cast<Red4 *>(red + (ks * BM + (wm * MT + t) * 16 + row16) * PITCH +
+                                          (wn * NF + f) * 16 + quad * 4) = acc[f][t];
+        __syncthreads();
+        const int nl = tid % (BN / 4) * 4, r0 = tid / (BN / 4);
+        if (n_base + nl >= N || r0 >= kPass) return;
+        for (int ml = r0; ml < tile.rows; ml += kPass) {
+            const int to = row_to[ml];
+            if (to < 0) continue;
+            Red4 sum = {0, 0, 0, 0};
+#pragma unroll
+            for (int q = 0; q < KS; ++q)
+                sum += *reinterpret_cast<const Red4 *>(red + (q * BM + ml) * PITCH + nl);
+            float v[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float s = float(sum[r]) * row_scale[ml];
+                v[r] = s * col_scale[nl + r];
+            }
+            *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p.y) + size_t(to) * N + n_base + nl) =
+                p.out_type == F16 ? uint2{pack2(v[0], v[1], f16_t{}), pack2(v[2], v[3], f16_t{})}
+                                  : uint2{pack2(v[0], v[1], bf16_t{}), pack2(v[2], v[3], bf16_t{})};
         }
-        *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p.y) + size_t(to) * N + n) = out;
     }
 }
 
 template <int Fmt, bool Grouped, int KS, int WN, int WM, int NF, int MT, int S, int EU>
 int launch(const ExpertArgs &a, hipStream_t stream) {
     constexpr int W = KS * WN * WM, BN = 16 * NF * WN, BM = 16 * MT * WM;
-    constexpr size_t ring = size_t(KS) * S * (BN + BM) * 128;
-    constexpr size_t lds = std::max(ring, size_t(KS) * BM * (BN + 4) * 4);
-    static_assert(lds <= size_t(kRing), "LDS");
+    constexpr size_t lds = expert_body_bytes(KS, S, BN, BM) + (2 * BM + BN) * 4;
+    static_assert(lds <= kLdsBytes, "LDS");
     const int tiles_n = (a.N + BN - 1) / BN;
     const int steps = ((a.K + 127) / 128 + KS - 1) / KS;
     hipLaunchKernelGGL((expert_gemm<Fmt, Grouped, KS, WN, WM, NF, MT, S, EU>),
