@@ -195,6 +195,9 @@ int qlin_expert_gemm(const qlin_path *path, const void *x, const float *sx, int 
     // tile's rows of either operand.
     if (order && long(x_rows) * K > INT32_MAX)
         return fail(QLIN_ERR_UNSUPPORTED, "gathered input rows exceed 2 GiB");
+    // So are the K groups' scales, the tokens' and one expert's.
+    if (group && (long(K) + 127) / 128 * (N > x_rows ? N : x_rows) * 4 > INT32_MAX)
+        return fail(QLIN_ERR_UNSUPPORTED, "K-group scale arrays exceed 2 GiB");
     int tile = choose_tile(slots, experts, N, K, fmt, group);
     if (path && path->kind) {
         tile = path->splits == 1 && path->staged == 0 ? tile_index(*path) : -1;

@@ -24,10 +24,15 @@ namespace qlin {
 #ifdef QLIN_EXPERT_PART
 namespace {
 
+// A stage: its rows and, with K groups, 1 KB of channel scales, the tokens' scales and
+// 256 bytes that surplus scale loads write.
+constexpr int expert_stage_bytes(bool grouped, int bn, int bm) {
+    return (bn + bm) * 128 + (grouped ? 1024 + (bm + 63) / 64 * 256 + 256 : 0);
+}
 // LDS of the slices' rings; afterwards of the partial tiles (one slice: of the
 // 16-bit results).
-constexpr int expert_body_bytes(int slices, int stages, int bn, int bm) {
-    const int ring = slices * stages * (bn + bm) * 128;
+constexpr int expert_body_bytes(bool grouped, int slices, int stages, int bn, int bm) {
+    const int ring = slices * stages * expert_stage_bytes(grouped, bn, bm);
     const int sums = slices == 1 ? bm * (bn + 8) * 2 : slices * bm * (bn + 4) * 4;
     return ring > sums ? ring : sums;
 }
@@ -45,7 +50,11 @@ __global__ __launch_bounds__(64 * KS * WN * WM, EU) void expert_gemm(ExpertArgs 
     using Acc = typename Mma::Acc;
     constexpr int NWS = WN * WM, W = KS * NWS;
     constexpr int BN = 16 * NF * WN, BM = 16 * MT * WM, BK = 128;
-    constexpr int STAGE = (BN + BM) * BK, WI = BN / 8 / NWS, XI = BM / 8 / NWS, INSTS = WI + XI;
+    constexpr int STAGE = expert_stage_bytes(Grouped, BN, BM);
+    // DMA instructions per wave and stage: weight rows, token rows and (K groups)
+    // scales, of which instruction 0 is the channels' and q the tokens [64 (q - 1), ..).
+    constexpr int SI = Grouped ? (1 + (BM + 63) / 64 + NWS - 1) / NWS : 0;
+    constexpr int WI = BN / 8 / NWS, XI = BM / 8 / NWS, INSTS = WI + XI + SI;
     static_assert(BN / 8 % NWS == 0 && BM / 8 % NWS == 0, "whole DMA instructions per wave");
     static_assert(S > 1 && (NWS == 1 || NWS % 2 == 0), "the ring refills behind its readers");
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
@@ -118,12 +127,6 @@ __global__ __launch_bounds__(64 * KS * WN * WM, EU) void expert_gemm(ExpertArgs 
         __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc_x, (lds_ptr_t)(dma_base + (BN / 8 + g) * 1024), 16, at,
                                                  dk, 0, 0);
     };
-    auto dma = [&](auto i_) {
-        constexpr int i = decltype(i_)::value;
-        if constexpr (i < WI) dma_w(std::integral_constant<int, i < WI ? i : 0>{});
-        else dma_x(std::integral_constant<int, i < WI ? 0 : i - WI>{});
-    };
-
     // Where all of a slice's stages fit its ring, their weights are asked for
     // before the rows' addresses are known (those wait for the offsets, then
     // the order).
@@ -146,45 +149,44 @@ __global__ __launch_bounds__(64 * KS * WN * WM, EU) void expert_gemm(ExpertArgs 
                                     uint32_t(chunk * 16);
     }
 
-    // K groups: the scales of a stage's group, two sets so that the next
-    // stage's arrive under this one's products.
-    struct Scales {
-        f32x4 w[Grouped ? NF : 1];
-        float x[Grouped ? MT : 1];
-    };
-    int sx_row[Grouped ? MT : 1];
-    if constexpr (Grouped) {
+    // K groups: a stage's scales arrive with it, [BN] then [BM] floats behind its
+    // rows, the tokens' gathered like the rows. Instructions that a wave has
+    // beside these write zeros behind them (all waves count the same loads).
+    const __amdgpu_buffer_rsrc_t rsrc_sw = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<float *>(sw + n_base), 0, Grouped ? (k_groups * N - n_base) * 4 : 0, 0x00020000);
+    const __amdgpu_buffer_rsrc_t rsrc_sx = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<float *>(p.sx), 0, Grouped ? k_groups * p.x_rows * 4 : 0, 0x00020000);
+    uint32_t soff[SI + 1];
 #pragma unroll
-        for (int t = 0; t < MT; ++t) sx_row[t] = max(source((wm * MT + t) * 16 + row16), 0);
+    for (int i = 0; i < SI; ++i) {
+        const int q = i * NWS + ws, ml = (q - 1) * 64 + lane;
+        const int row = q > 0 && ml < BM ? source(ml) : -1;
+        soff[i] = q == 0 ? (lane * 4 < BN && n_base + lane * 4 < N ? uint32_t(lane * 16) : kOut)
+                  : row < 0 ? kOut : uint32_t(row) * 4u;
     }
-    auto load_scales = [&](int st, Scales &s) {
-        if constexpr (Grouped) {
-            const int g = min(k_begin / BK + st, k_groups - 1);
-#pragma unroll
-            for (int f = 0; f < NF; ++f) {
-                const int n = min(n_base + (wn * NF + f) * 16 + quad * 4, N - 4);
-                s.w[f] = *reinterpret_cast<const f32x4 *>(sw + size_t(g) * N + n);
-            }
-#pragma unroll
-            for (int t = 0; t < MT; ++t) s.x[t] = p.sx[size_t(g) * p.x_rows + sx_row[t]];
-            if constexpr (KS > 1 && NWS > 1) {
-                // A slice's stages past K add zeros, whatever the last group's scales are.
-                const bool live = k_begin / BK + st < k_groups;
-#pragma unroll
-                for (int f = 0; f < NF; ++f)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) s.w[f][r] = live ? s.w[f][r] : 0.f;
-#pragma unroll
-                for (int t = 0; t < MT; ++t) s.x[t] = live ? s.x[t] : 0.f;
-            }
+    auto dma_s = [&](auto i_) {
+        constexpr int i = decltype(i_)::value;
+        const uint32_t g = dk / BK, at = int(g) < k_groups ? soff[i] : kOut;
+        const int q = i * NWS + ws;
+        uint8_t *dst = dma_base + (BN + BM) * BK;
+        if (q == 0) {
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc_sw, (lds_ptr_t)dst, 16, at, g * uint32_t(N) * 4u, 0, 0);
+        } else {
+            dst += 1024 + min(q - 1, (BM + 63) / 64) * 256;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc_sx, (lds_ptr_t)dst, 4, at,
+                                                     g * uint32_t(p.x_rows) * 4u, 0, 0);
         }
     };
-    Scales s0, s1;
-    load_scales(0, s0);
+    auto dma = [&](auto i_) {
+        constexpr int i = decltype(i_)::value;
+        if constexpr (i < WI) dma_w(std::integral_constant<int, i < WI ? i : 0>{});
+        else if constexpr (i < WI + XI) dma_x(std::integral_constant<int, i < WI ? 0 : i - WI>{});
+        else dma_s(std::integral_constant<int, i < WI + XI ? 0 : i - WI - XI>{});
+    };
 
     // For the epilogue, in LDS past the ring: the rows' scales and where they go, the
     // channels' scales.
-    constexpr int kBody = expert_body_bytes(KS, S, BN, BM);
+    constexpr int kBody = expert_body_bytes(Grouped, KS, S, BN, BM);
     float *row_scale = reinterpret_cast<float *>(lds + kBody), *col_scale = row_scale + BM;
     int *row_to = reinterpret_cast<int *>(col_scale + BN);
     for (int i = tid; i < BM; i += 64 * W) {
@@ -214,22 +216,37 @@ __global__ __launch_bounds__(64 * KS * WN * WM, EU) void expert_gemm(ExpertArgs 
         const i32x4 hi = *reinterpret_cast<const i32x4 *>(q + c1);
         return i32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
     };
-    auto read_x = [&](int slot, i32x8 (&b)[MT]) {
+    auto read_x = [&](int slot, auto &b) {
 #pragma unroll
-        for (int t = 0; t < MT; ++t) b[t] = frag(slot, BN + (wm * MT + t) * 16);
+        for (int t = 0; t < int(sizeof(b) / sizeof(b[0])); ++t) b[t] = frag(slot, BN + (t * WM + wm) * 16);
     };
     auto read_w = [&](int slot, int f) { return frag(slot, (wn * NF + f) * 16); };
+    // The scales of a weight fragment's channels and of the wave's tokens.
+    auto read_sw = [&](int slot, int f) {
+        if constexpr (Grouped)
+            return *reinterpret_cast<const f32x4 *>(ring + slot * STAGE + (BN + BM) * BK +
+                                                    ((wn * NF + f) * 16 + quad * 4) * 4);
+        else
+            return f32x4{};
+    };
+    auto read_sx = [&](int slot, auto &s) {
+        if constexpr (Grouped) {
+            const float *q = reinterpret_cast<const float *>(ring + slot * STAGE + (BN + BM) * BK + 1024);
+#pragma unroll
+            for (int t = 0; t < int(sizeof(s) / sizeof(s[0])); ++t) s[t] = q[(t * WM + wm) * 16 + row16];
+        }
+    };
     // Products of weight fragment f with the stage's token fragments.
-    auto row = [&](auto f_, const i32x8 &a, const i32x8 (&b)[MT], const Scales &s) {
+    auto row = [&](auto f_, const i32x8 &a, const f32x4 &aw, const auto &b, const auto &bx) {
         constexpr int f = decltype(f_)::value;
 #pragma unroll
-        for (int t = 0; t < MT; ++t) {
+        for (int t = 0; t < int(sizeof(b) / sizeof(b[0])); ++t) {
             if constexpr (Grouped) {
                 Acc part = Acc{0, 0, 0, 0};
                 Mma::run(part, a, b[t]);
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
-                    acc[f][t][r] = __builtin_fmaf(float(part[r]), s.x[t] * s.w[f][r], acc[f][t][r]);
+                    acc[f][t][r] = __builtin_fmaf(float(part[r]), bx[t] * aw[r], acc[f][t][r]);
             } else {
                 Mma::run(acc[f][t], a, b[t]);
             }
@@ -244,13 +261,14 @@ __global__ __launch_bounds__(64 * KS * WN * WM, EU) void expert_gemm(ExpertArgs 
             aim(s, s);
             if (!whole) static_for<0, WI>(dma_w);
             static_for<0, XI>(dma_x);
+            static_for<0, SI>(dma_s);
         }
     // Wait for stage `st` with `newer` later ones asked for.
     auto wait_stage = [&](int newer) {
         if (whole) {
-            if (newer >= 3 && S > 3) wait_vmcnt<XI * 3>();
-            else if (newer == 2) wait_vmcnt<XI * 2>();
-            else if (newer == 1) wait_vmcnt<XI>();
+            if (newer >= 3 && S > 3) wait_vmcnt<(XI + SI) * 3>();
+            else if (newer == 2) wait_vmcnt<(XI + SI) * 2>();
+            else if (newer == 1) wait_vmcnt<XI + SI>();
             else wait_vmcnt<0>();
         } else {
             if (newer >= 3 && S > 3) wait_vmcnt<INSTS * 3>();
@@ -266,17 +284,16 @@ __global__ __launch_bounds__(64 * KS * WN * WM, EU) void expert_gemm(ExpertArgs 
     // fragments are read one 16-row block ahead of their MFMAs, the next stage's
     // token fragments and first weight fragment under the last block's, once
     // that stage has landed (with a shared ring for every wave: the barrier).
-    auto step = [&](int s, i32x8 &a, const i32x8 (&b)[MT], const Scales &sc, i32x8 (&nb)[MT],
-                    Scales &nsc) {
-        load_scales(s + 1, nsc);
+    auto step = [&](int s, i32x8 &a, f32x4 &aw, const auto &b, const auto &bx, auto &nb, auto &nbx) {
         if (s > 0 && s - 1 + S < count) {
             aim(s - 1 + S, slot == 0 ? S - 1 : slot - 1);
             static_for<0, INSTS>(dma);
         }
         static_for<0, NF - 1>([&](auto f_) {
             const i32x8 an = read_w(slot, decltype(f_)::value + 1);
-            row(f_, a, b, sc);
-            a = an;
+            const f32x4 anw = read_sw(slot, decltype(f_)::value + 1);
+            row(f_, a, aw, b, bx);
+            a = an, aw = anw;
             pin();  // (a stage's weight fragments at once do not fit the registers)
         });
         slot = slot + 1 == S ? 0 : slot + 1;
@@ -288,24 +305,50 @@ __global__ __launch_bounds__(64 * KS * WN * WM, EU) void expert_gemm(ExpertArgs 
         // (After the last stage a slot whose fragments go unused: a conditional
         // read would copy every fragment.)
         read_x(slot, nb);
+        read_sx(slot, nbx);
         const i32x8 an = read_w(slot, 0);
-        row(std::integral_constant<int, NF - 1>{}, a, b, sc);
-        a = an;
+        const f32x4 anw = read_sw(slot, 0);
+        row(std::integral_constant<int, NF - 1>{}, a, aw, b, bx);
+        a = an, aw = anw;
     };
-    i32x8 a, b0[MT], b1[MT];
-    if (count > 0) {
+    // All stages for the wave's first L token fragments.
+    auto walk = [&](auto live_) {
+        constexpr int L = decltype(live_)::value;
+        i32x8 a, b0[L], b1[L];
+        f32x4 aw;
+        float x0[L], x1[L];
         wait_stage(min(S, count) - 1);
         if constexpr (NWS > 1) __builtin_amdgcn_s_barrier();
         pin();
         read_x(0, b0);
+        read_sx(0, x0);
         a = read_w(0, 0);
+        aw = read_sw(0, 0);
         int s = 0;
         for (; s + 1 < count; s += 2) {
-            step(s, a, b0, s0, b1, s1);
-            step(s + 1, a, b1, s1, b0, s0);
+            step(s, a, aw, b0, x0, b1, x1);
+            step(s + 1, a, aw, b1, x1, b0, x0);
         }
-        if (s < count) step(s, a, b0, s0, b1, s1);
+        if (s < count) step(s, a, aw, b0, x0, b1, x1);
+    };
+    // The waves along the tokens take the tile's 16-row fragments in turn, so a
+    // group's short last tile has fewer in every wave, and only those are
+    // multiplied (4096 tokens x 4 of 32 experts, 4096 x 2048 INT8: @LIVE@).
+    const int live = (tile.rows - wm * 16 + 16 * WM - 1) / (16 * WM);
+    if (count > 0) {
+        if constexpr (MT >= 4) {
+            if (live >= 4) walk(std::integral_constant<int, 4>{});
+            else if (live == 3) walk(std::integral_constant<int, 3>{});
+            else if (live == 2) walk(std::integral_constant<int, 2>{});
+            else walk(std::integral_constant<int, 1>{});
+        } else if constexpr (MT == 2) {
+            if (live >= 2) walk(std::integral_constant<int, 2>{});
+            else walk(std::integral_constant<int, 1>{});
+        } else {
+            walk(std::integral_constant<int, MT>{});
+        }
     }
+    static_assert(MT == 1 || MT == 2 || MT == 4, "the walks above");
     wait_lds_reads();
     __syncthreads();
 
@@ -318,7 +361,7 @@ __global__ __launch_bounds__(64 * KS * WN * WM, EU) void expert_gemm(ExpertArgs 
         uint16_t *tile16 = reinterpret_cast<uint16_t *>(lds);
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
-            const int ml = (wm * MT + t) * 16 + row16;
+            const int ml = (t * WM + wm) * 16 + row16;
             const float scale_x = row_scale[ml];
 #pragma unroll
             for (int f = 0; f < NF; ++f) {
@@ -362,7 +405,7 @@ __global__ __launch_bounds__(64 * KS * WN * WM, EU) void expert_gemm(ExpertArgs 
         for (int t = 0; t < MT; ++t)
 #pragma unroll
             for (int f = 0; f < NF; ++f)
-                *reinterpret_cast<Red4 *>(red + (ks * BM + (wm * MT + t) * 16 + row16) * PITCH +
+                *reinterpret_cast<Red4 *>(red + (ks * BM + (t * WM + wm) * 16 + row16) * PITCH +
                                           (wn * NF + f) * 16 + quad * 4) = acc[f][t];
         __syncthreads();
         const int nl = tid % (BN / 4) * 4, r0 = tid / (BN / 4);
@@ -390,7 +433,7 @@ __global__ __launch_bounds__(64 * KS * WN * WM, EU) void expert_gemm(ExpertArgs 
 template <int Fmt, bool Grouped, int KS, int WN, int WM, int NF, int MT, int S, int EU>
 int launch(const ExpertArgs &a, hipStream_t stream) {
     constexpr int W = KS * WN * WM, BN = 16 * NF * WN, BM = 16 * MT * WM;
-    constexpr size_t lds = expert_body_bytes(KS, S, BN, BM) + (2 * BM + BN) * 4;
+    constexpr size_t lds = expert_body_bytes(Grouped, KS, S, BN, BM) + (2 * BM + BN) * 4;
     static_assert(lds <= kLdsBytes, "LDS");
     const int tiles_n = (a.N + BN - 1) / BN;
     const int steps = ((a.K + 127) / 128 + KS - 1) / KS;

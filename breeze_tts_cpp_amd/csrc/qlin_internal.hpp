@@ -190,21 +190,21 @@ struct ExpertArgs {
 // Macro tiles: index, K slices, waves along channels and tokens, 16-row
 // fragments per wave of both, LDS stages, waves per SIMD.
 #define QLIN_EXPERT_TILES(X)   \
-    X(0, 8, 1, 1, 1, 1, 4, 2)  \
-    X(1, 8, 1, 1, 2, 1, 3, 2)  \
+    X(0, 1, 2, 1, 4, 1, 3, 2)  \
+    X(1, 1, 2, 1, 2, 1, 4, 2)  \
     X(2, 4, 1, 1, 2, 1, 3, 2)  \
     X(3, 4, 1, 1, 4, 1, 3, 1)  \
-    X(4, 4, 1, 1, 2, 2, 4, 1)  \
+    X(4, 1, 4, 1, 2, 2, 2, 4)  \
     X(5, 2, 2, 2, 2, 2, 2, 4)  \
     X(6, 1, 2, 4, 4, 2, 2, 4)  \
     X(7, 1, 4, 2, 4, 4, 3, 2)  \
     X(8, 1, 2, 2, 2, 2, 2, 4)  \
-    X(9, 1, 4, 2, 4, 2, 2, 4)  \
+    X(9, 1, 4, 1, 1, 2, 3, 4)  \
     X(10, 1, 4, 2, 2, 2, 3, 4) \
-    X(11, 4, 1, 1, 1, 1, 4, 4) \
-    X(12, 4, 1, 1, 4, 2, 2, 2) \
+    X(11, 2, 2, 1, 2, 1, 3, 2) \
+    X(12, 1, 4, 2, 2, 2, 2, 4) \
     X(13, 1, 2, 4, 8, 4, 2, 2) \
-    X(14, 8, 1, 1, 2, 2, 2, 2) \
+    X(14, 1, 4, 1, 2, 4, 2, 3) \
     X(15, 1, 4, 1, 2, 2, 3, 3) \
     X(16, 1, 2, 4, 4, 2, 3, 2)
 struct ExpertTile {

@@ -30,8 +30,11 @@ struct RowTile {
 
 // The tile of workgroup `index`: the groups' row tiles of at most `height`
 // slots times `columns` column tiles, numbered group by group, each column
-// tile's row tiles in a run (they share the group's weights there), placed
-// XCD-major. False past the last tile. Offsets are held to [0, slots] and
+// tile's row tiles in a run (they share the group's weights there). The
+// hardware places workgroup i on XCD i % 8: every 256 workgroups (a round of the
+// CUs) take 256 tiles, each XCD 32 in a run that share its L2; the rest of the
+// tiles is numbered XCD-major. (All tiles XCD-major puts whole groups on one XCD,
+// and groups differ in size: @XCD@.) False past the last tile. Offsets are held to [0, slots] and
 // ascending order here, so bad ones cannot lead out of the arrays. Same
 // result in every lane of the workgroup.
 __device__ __forceinline__ bool find_tile(const int *__restrict__ offsets, int groups, int slots,
@@ -51,7 +54,9 @@ __device__ __forceinline__ bool find_tile(const int *__restrict__ offsets, int g
     }
     const int total = __builtin_amdgcn_readlane(wave_scan(mine), 63) * columns;
     if (index >= total) return false;
-    const int at = xcd_major(index, total);
+    const int whole = total & ~255;
+    const int at = index < whole ? (index & ~255) + (index % 8) * 32 + index % 256 / 8
+                                 : whole + xcd_major(index - whole, total - whole);
     int before = 0;  // row tiles of the groups before this run of 64
     for (int g0 = 0; g0 < groups; g0 += 64) {
         int begin = first_begin;
