@@ -64,52 +64,62 @@ __device__ __forceinline__ int group_rank(const AdapterArgs &p, int g) {
     return p.ranks ? min(max(p.ranks[g], 0), p.rank) : p.rank;
 }
 
-// acc[i][t] += A rows [16i, 16i + 16) x the tile's tokens [16t, 16t + 16) over the K
-// range [k0, k1) (32 at a time; k0 a multiple of 32).
-template <class T, int RT, int MT, bool Vec>
-__device__ __forceinline__ void shrink(const AdapterArgs &p, const RowTile &tile, int rank, int k0,
-                                       int k1, f32x4 (&acc)[RT][MT]) {
+// acc[i] += A rows [16 i, 16 i + 16) x the tile's 16 tokens over K [k0, k1). A block is 64 K: a
+// lane takes 16 of them for two MFMAs (both operands in the same order), so its
+// two loads and its row's four lanes cover a whole 128-byte line. `Deep` blocks
+// are asked for ahead of the ones multiplied.
+template <class T, int RT, int Deep, bool Vec>
+__device__ __forceinline__ void shrink(const AdapterArgs &p, const RowTile &tile, int rank, int row,
+                                       int k0, int k1, f32x4 (&acc)[RT]) {
     const int lane = threadIdx.x & 63, row16 = lane & 15, quad = lane >> 4;
-    const uint16_t *xrow[MT], *arow[RT];
-    bool xin[MT], ain[RT];
-#pragma unroll
-    for (int t = 0; t < MT; ++t) {
-        const int row = source_row(p, tile, t * 16 + row16);
-        xin[t] = row >= 0;
-        xrow[t] = static_cast<const uint16_t *>(p.x) + size_t(max(row, 0)) * p.ldx + quad * 8;
-    }
+    const uint16_t *xrow = static_cast<const uint16_t *>(p.x) + size_t(max(row, 0)) * p.ldx;
+    const uint16_t *arow[RT];
+    bool ain[RT];
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
         const int r = i * 16 + row16;
         ain[i] = r < rank;
         arow[i] = static_cast<const uint16_t *>(p.a) +
-                  (size_t(tile.group) * p.rank + min(r, p.rank - 1)) * p.K + quad * 8;
+                  (size_t(tile.group) * p.rank + min(r, p.rank - 1)) * p.K;
     }
-    // kDeep steps' loads are issued together, then their products.
-    constexpr int kDeep = RT * MT >= 16 ? 1 : RT + MT >= 6 ? 2 : 4;
-    for (int k = k0; k < k1; k += 32 * kDeep) {
-        uint4 xv[kDeep][MT], av[kDeep][RT];
+    struct Block {
+        uint4 x[2], a[RT][2];
+    };
+    // Pieces past the range come from the row's start and count as zeros.
+    auto load = [&](int k, Block &o) {
 #pragma unroll
-        for (int d = 0; d < kDeep; ++d) {
-            const bool in = k + d * 32 + quad * 8 < k1;
-            const int at = in ? k + d * 32 : -quad * 8;  // (past the range: the row's start)
-#pragma unroll
-            for (int t = 0; t < MT; ++t) {
-                const uint4 v = load_piece<Vec>(xrow[t] + at, 8);
-                xv[d][t] = in && xin[t] ? v : uint4{0, 0, 0, 0};
-            }
+        for (int h = 0; h < 2; ++h) {
+            const int at = k + quad * 16 + h * 8;
+            const bool in = at < k1;
+            const uint4 none = uint4{0, 0, 0, 0};
+            const uint4 xv = load_piece<Vec>(xrow + (in ? at : 0), 8);
+            o.x[h] = in && row >= 0 ? xv : none;
 #pragma unroll
             for (int i = 0; i < RT; ++i) {
-                const uint4 v = load_piece<true>(arow[i] + at, 8);
-                av[d][i] = in && ain[i] ? v : uint4{0, 0, 0, 0};
+                const uint4 av = load_piece<true>(arow[i] + (in ? at : 0), 8);
+                o.a[i][h] = in && ain[i] ? av : none;
             }
         }
+    };
+    auto multiply = [&](const Block &o) {
 #pragma unroll
-        for (int d = 0; d < kDeep; ++d)
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int i = 0; i < RT; ++i)
+            for (int i = 0; i < RT; ++i) mma16<T>(acc[i], o.a[i][h], o.x[h]);
+    };
+    Block now[Deep], next[Deep];
 #pragma unroll
-                for (int t = 0; t < MT; ++t) mma16<T>(acc[i][t], av[d][i], xv[d][t]);
+    for (int d = 0; d < Deep; ++d) load(k0 + d * 64, now[d]);
+    for (int k = k0; k < k1; k += Deep * 64) {
+        const bool more = k + Deep * 64 < k1;
+        if (more) {
+#pragma unroll
+            for (int d = 0; d < Deep; ++d) load(k + (Deep + d) * 64, next[d]);
+        }
+#pragma unroll
+        for (int d = 0; d < Deep; ++d) multiply(now[d]);
+#pragma unroll
+        for (int d = 0; d < Deep; ++d) now[d] = next[d];
     }
 }
 
@@ -144,234 +154,149 @@ __device__ __forceinline__ void split_token(const float (&t)[RP / 16], uint16_t 
     if (l == 0) *exponent = e;
 }
 
-// The second product for channels [n0, n0 + 32) and the tile's tokens, added to
-// base and stored. hi / lo: [16 MT][RP + 8] in LDS. MFMA row p of fragment f
-// is channel 8 (p / 4) + 4 f + p % 4 of the 32, so a lane's two fragments are
-// eight consecutive channels.
-template <class T, int RP, int MT, bool VecB, bool VecY>
-__device__ __forceinline__ void expand(const AdapterArgs &p, const RowTile &tile, int rank, int n0,
-                                       const uint16_t *hi, const uint16_t *lo, const int *exponent,
-                                       float scale) {
+// What the second product reads for channels [n0, n0 + 32): B's rows and the
+// base. MFMA row p of fragment f is channel 8 (p / 4) + 4 f + p % 4 of the 32,
+// so a lane's two fragments are eight consecutive channels of its token.
+template <int RP> struct Panel {
+    uint4 b[2][RP / 32], base;
+};
+template <class T, int RP, bool VecB, bool VecY>
+__device__ __forceinline__ void load_panel(const AdapterArgs &p, const RowTile &tile, int rank, int row,
+                                           int n0, Panel<RP> &o) {
     const int lane = threadIdx.x & 63, row16 = lane & 15, quad = lane >> 4;
-    constexpr int kSteps = RP / 32, kPitch = RP + 8;
-    uint4 bv[2][kSteps];
 #pragma unroll
     for (int f = 0; f < 2; ++f) {
         const int n = n0 + 8 * (row16 / 4) + 4 * f + row16 % 4;
-        const uint16_t *row = static_cast<const uint16_t *>(p.b) +
-                              (size_t(tile.group) * p.N + min(n, p.N - 1)) * p.rank;
+        const uint16_t *at = static_cast<const uint16_t *>(p.b) +
+                             (size_t(tile.group) * p.N + min(n, p.N - 1)) * p.rank;
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
+        for (int s = 0; s < RP / 32; ++s) {
             const int r = s * 32 + quad * 8;
             const int have = n < p.N ? min(rank - r, 8) : 0;
-            bv[f][s] = have > 0 ? load_piece<VecB>(row + r, have) : uint4{0, 0, 0, 0};
+            o.b[f][s] = have > 0 ? load_piece<VecB>(at + r, have) : uint4{0, 0, 0, 0};
         }
     }
-#pragma unroll
-    for (int t = 0; t < MT; ++t) {
-        const int ml = t * 16 + row16, row = source_row(p, tile, ml), n = n0 + quad * 8;
-        const bool live = row >= 0 && n < p.N;
-        const size_t at = size_t(max(row, 0)) * p.ldy + n;
-        float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-        if (live && p.base)
-            load8<T, VecY>(static_cast<const uint16_t *>(p.base) + at, 0, 8, v);
-        f32x4 acc[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-            const uint4 h = *reinterpret_cast<const uint4 *>(hi + ml * kPitch + s * 32 + quad * 8);
-            const uint4 l = *reinterpret_cast<const uint4 *>(lo + ml * kPitch + s * 32 + quad * 8);
-#pragma unroll
-            for (int f = 0; f < 2; ++f) {
-                mma16<T>(acc[f], bv[f][s], l);
-                mma16<T>(acc[f], bv[f][s], h);
-            }
-        }
-        const int e = exponent[ml];
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            v[i] += scale * __builtin_amdgcn_ldexpf(acc[i / 4][i % 4], e);
-        if (live) store16x8<T, VecY>(static_cast<uint16_t *>(p.y) + at, 0, 8, v);
-    }
-}
-
-// t of a tile from the waves' partial sums in LDS ([parts][16 MT][RP]; they
-// may be the workspace's, part_stride floats apart) to hi / lo.
-template <class T, int RP, int MT>
-__device__ __forceinline__ void gather_t(const float *parts, int count, size_t part_stride,
-                                         int live_rows, int rank, uint16_t *hi, uint16_t *lo,
-                                         int *exponent) {
-    for (int ml = threadIdx.x / 16; ml < 16 * MT; ml += blockDim.x / 16) {
-        float t[RP / 16];
-#pragma unroll
-        for (int i = 0; i < RP / 16; ++i) t[i] = 0.f;
-        if (ml < live_rows)
-            for (int q = 0; q < count; ++q)
-#pragma unroll
-                for (int i = 0; i < RP / 16; ++i)
-                    t[i] += parts[q * part_stride + size_t(ml) * RP + i * 16 + threadIdx.x % 16];
-        // (Past the rank A was read as zeros, but 0 * inf is NaN.)
-#pragma unroll
-        for (int i = 0; i < RP / 16; ++i)
-            if (i * 16 + int(threadIdx.x % 16) >= rank) t[i] = 0.f;
-        split_token<T, RP>(t, hi + ml * (RP + 8), lo + ml * (RP + 8), exponent + ml);
-    }
+    const int n = n0 + quad * 8;
+    o.base = uint4{0, 0, 0, 0};
+    if (p.base && row >= 0 && n < p.N)
+        o.base = load_raw8<VecY>(static_cast<const uint16_t *>(p.base) + size_t(row) * p.ldy + n, 0, 8);
 }
 
 constexpr int rank_pad(int rt) { return rt < 2 ? 32 : 16 * rt; }
+constexpr int kAdapterWaves = 8, kAdapterThreads = 64 * kAdapterWaves;
 
-// ---------------------------------------------------------------- one launch
-// A 16-row tile's whole work in one workgroup: its eight waves split K of the
-// first product, sum through LDS, and split the tile's channels of the second.
-// Every column tile of the same rows repeats the first product.
+// One workgroup: 16 rows of one adapter, `width` channels. Its eight waves split
+// K of the first product, sum t through LDS, split it into hi and lo there, and
+// take 32 channels at a time of the second, the next 32's operands (the first
+// ones from the start) asked for ahead. Column tiles of the same rows repeat the
+// first product.
 template <class T, int RT, bool VecX, bool VecB, bool VecY>
-__global__ __launch_bounds__(512) void adapter_one(AdapterArgs p, int columns, int width) {
-    constexpr int RP = rank_pad(RT), W = 8;
+__global__ __launch_bounds__(kAdapterThreads) void adapter_rows(AdapterArgs p, int columns, int width) {
+    constexpr int RP = rank_pad(RT), W = kAdapterWaves, kPitch = RP + 8;
+    constexpr int Deep = RT >= 4 ? 1 : RT == 2 ? 2 : 4;
     __shared__ __attribute__((aligned(16))) float parts[W * 16 * RP];
-    __shared__ __attribute__((aligned(16))) uint16_t hi[16 * (RP + 8)], lo[16 * (RP + 8)];
+    __shared__ __attribute__((aligned(16))) uint16_t hi[16 * kPitch], lo[16 * kPitch];
     __shared__ int exponent[16];
     RowTile tile;
     if (!find_tile(p.offsets, p.adapters, p.rows, 16, columns, blockIdx.x, tile)) return;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row16 = lane & 15, quad = lane >> 4;
+    const int lane = threadIdx.x & 63, row16 = lane & 15, quad = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int rank = group_rank(p, tile.group);
     const float scale = p.scales ? p.scales[tile.group] : 1.f;
-    f32x4 acc[RT][1];
+    const int row = source_row(p, tile, row16);
+    const int n_first = tile.column * width + wave * 32;
+    const int n_end = min((tile.column + 1) * width, p.N);
+    Panel<RP> now, next;
+    load_panel<T, RP, VecB, VecY>(p, tile, rank, row, min(n_first, p.N - 1), now);
+
+    f32x4 acc[RT];
 #pragma unroll
-    for (int i = 0; i < RT; ++i) acc[i][0] = f32x4{0, 0, 0, 0};
-    const int span = ((p.K + 31) / 32 + W - 1) / W * 32;
-    shrink<T, RT, 1, VecX>(p, tile, rank, min(wave * span, p.K), min((wave + 1) * span, p.K), acc);
+    for (int i = 0; i < RT; ++i) acc[i] = f32x4{0, 0, 0, 0};
+    const int span = ((p.K + 63) / 64 + W - 1) / W * 64;
+    const int k0 = min(wave * span, p.K);
+    shrink<T, RT, Deep, VecX>(p, tile, rank, row, k0, min(k0 + span, p.K), acc);
 #pragma unroll
     for (int i = 0; i < RP / 16; ++i)
         *reinterpret_cast<f32x4 *>(parts + (wave * 16 + row16) * RP + i * 16 + quad * 4) =
-            i < RT ? acc[i < RT ? i : 0][0] : f32x4{0, 0, 0, 0};
+            i < RT ? acc[i < RT ? i : 0] : f32x4{0, 0, 0, 0};
     __syncthreads();
-    gather_t<T, RP, 1>(parts, W, 16 * RP, 16, rank, hi, lo, exponent);
-    __syncthreads();
-    const int n_end = min((tile.column + 1) * width, p.N);
-    for (int n0 = tile.column * width + wave * 32; n0 < n_end; n0 += W * 32)
-        expand<T, RP, 1, VecB, VecY>(p, tile, rank, n0, hi, lo, exponent, scale);
-}
-
-// ---------------------------------------------------------------- two launches
-// First product: a 64-row tile's K range split over the grid and four waves;
-// partial t [split][slot][RP] to the workspace.
-template <class T, int RT, bool VecX>
-__global__ __launch_bounds__(256) void adapter_shrink(AdapterArgs p, int splits) {
-    constexpr int RP = rank_pad(RT), W = 4, MT = 4;
-    __shared__ __attribute__((aligned(16))) float parts[W * 16 * RP];
-    RowTile tile;
-    if (!find_tile(p.offsets, p.adapters, p.rows, 16 * MT, splits, blockIdx.x, tile)) return;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row16 = lane & 15, quad = lane >> 4;
-    const int rank = group_rank(p, tile.group);
-    f32x4 acc[RT][MT];
+    if (threadIdx.x < 256) {  // 16 lanes per token
+        const int ml = threadIdx.x / 16, l = threadIdx.x % 16;
+        float t[RP / 16];
 #pragma unroll
-    for (int i = 0; i < RT; ++i)
+        for (int i = 0; i < RP / 16; ++i) {
+            t[i] = 0.f;
 #pragma unroll
-        for (int t = 0; t < MT; ++t) acc[i][t] = f32x4{0, 0, 0, 0};
-    const int ranges = W * splits, span = ((p.K + 31) / 32 + ranges - 1) / ranges * 32;
-    const int k0 = min((tile.column * W + wave) * span, p.K);
-    shrink<T, RT, MT, VecX>(p, tile, rank, k0, min(k0 + span, p.K), acc);
-    float *out = static_cast<float *>(p.workspace) +
-                 (size_t(tile.column) * p.rows + tile.begin) * RP;
-#pragma unroll
-    for (int t = 0; t < MT; ++t) {
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < RP / 16; ++i)
-            *reinterpret_cast<f32x4 *>(parts + (wave * 16 + row16) * RP + i * 16 + quad * 4) =
-                i < RT ? acc[i < RT ? i : 0][t] : f32x4{0, 0, 0, 0};
-        __syncthreads();
-        for (int i = threadIdx.x; i < 16 * RP; i += 256) {
-            if (t * 16 + i / RP >= tile.rows) break;
-            float s = 0.f;
-#pragma unroll
-            for (int q = 0; q < W; ++q) s += parts[q * 16 * RP + i];
-            out[size_t(t) * 16 * RP + i] = s;
+            for (int q = 0; q < W; ++q) t[i] += parts[(q * 16 + ml) * RP + i * 16 + l];
+            // (Past the rank A was read as zeros, but 0 * inf is NaN.)
+            if (i * 16 + l >= rank) t[i] = 0.f;
         }
+        split_token<T, RP>(t, hi + ml * kPitch, lo + ml * kPitch, exponent + ml);
     }
-}
-
-template <class T, int RT, bool VecB, bool VecY>
-__global__ __launch_bounds__(256) void adapter_expand(AdapterArgs p, int splits, int columns,
-                                                      int width) {
-    constexpr int RP = rank_pad(RT), MT = 4, W = 4;
-    __shared__ __attribute__((aligned(16))) uint16_t hi[64 * (RP + 8)], lo[64 * (RP + 8)];
-    __shared__ int exponent[64];
-    RowTile tile;
-    if (!find_tile(p.offsets, p.adapters, p.rows, 16 * MT, columns, blockIdx.x, tile)) return;
-    const int wave = threadIdx.x >> 6;
-    const int rank = group_rank(p, tile.group);
-    const float scale = p.scales ? p.scales[tile.group] : 1.f;
-    gather_t<T, RP, MT>(static_cast<const float *>(p.workspace) + size_t(tile.begin) * RP, splits,
-                        size_t(p.rows) * RP, tile.rows, rank, hi, lo, exponent);
     __syncthreads();
-    const int n_end = min((tile.column + 1) * width, p.N);
-    for (int n0 = tile.column * width + wave * 32; n0 < n_end; n0 += W * 32)
-        expand<T, RP, MT, VecB, VecY>(p, tile, rank, n0, hi, lo, exponent, scale);
-}
-
-struct AdapterPlan {
-    bool one;
-    int splits, columns, width;
-};
-AdapterPlan plan_adapter(int rows, int adapters, int N, int K, int rank) {
-    (void)rank;
-    AdapterPlan p{};
-    p.one = rows <= 64;
-    const long tiles = expert_row_tiles(rows, adapters, p.one ? 16 : 64);
-    const long wanted = std::max(1L, (p.one ? 256 : 512) / tiles);
-    const int unit = p.one ? 256 : 128;
-    p.columns = int(std::min(wanted, long(N + unit - 1) / unit));
-    p.width = ((N + unit - 1) / unit + p.columns - 1) / p.columns * unit;
-    p.columns = (N + p.width - 1) / p.width;
-    p.splits = p.one ? 0 : int(std::min(std::min(wanted, 8L), long(K + 255) / 256));
-    return p;
+    uint4 h[RP / 32], l[RP / 32];
+#pragma unroll
+    for (int s = 0; s < RP / 32; ++s) {
+        h[s] = *reinterpret_cast<const uint4 *>(hi + row16 * kPitch + s * 32 + quad * 8);
+        l[s] = *reinterpret_cast<const uint4 *>(lo + row16 * kPitch + s * 32 + quad * 8);
+    }
+    const int e = exponent[row16];
+    for (int n0 = n_first; n0 < n_end; n0 += W * 32) {
+        if (n0 + W * 32 < n_end) load_panel<T, RP, VecB, VecY>(p, tile, rank, row, n0 + W * 32, next);
+        f32x4 out[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
+#pragma unroll
+        for (int s = 0; s < RP / 32; ++s)
+#pragma unroll
+            for (int f = 0; f < 2; ++f) {
+                mma16<T>(out[f], now.b[f][s], l[s]);
+                mma16<T>(out[f], now.b[f][s], h[s]);
+            }
+        float v[8];
+        widen8<T>(now.base, v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] += scale * __builtin_amdgcn_ldexpf(out[i / 4][i % 4], e);
+        const int n = n0 + quad * 8;
+        if (row >= 0 && n < p.N)
+            store16x8<T, VecY>(static_cast<uint16_t *>(p.y) + size_t(row) * p.ldy + n, 0, 8, v);
+        now = next;
+    }
 }
 
 template <class T, int RT, bool VecX, bool VecB, bool VecY>
-void launch_as(const AdapterArgs &a, const AdapterPlan &p, hipStream_t s) {
-    const int tiles = int(expert_row_tiles(a.rows, a.adapters, p.one ? 16 : 64));
-    if (p.one) {
-        hipLaunchKernelGGL((adapter_one<T, RT, VecX, VecB, VecY>), dim3(unsigned(tiles * p.columns)),
-                           dim3(512), 0, s, a, p.columns, p.width);
-        return;
-    }
-    hipLaunchKernelGGL((adapter_shrink<T, RT, VecX>), dim3(unsigned(tiles * p.splits)), dim3(256), 0,
-                       s, a, p.splits);
-    hipLaunchKernelGGL((adapter_expand<T, RT, VecB, VecY>), dim3(unsigned(tiles * p.columns)),
-                       dim3(256), 0, s, a, p.splits, p.columns, p.width);
+void launch_as(const AdapterArgs &a, hipStream_t s) {
+    // Column tiles until the row tiles fill the CUs, of at least 256 channels.
+    const long tiles = expert_row_tiles(a.rows, a.adapters, 16);
+    const int units = (a.N + 255) / 256;
+    const int wanted = int(std::max(1L, std::min(256 / tiles, long(units))));
+    const int width = (units + wanted - 1) / wanted * 256, columns = (a.N + width - 1) / width;
+    hipLaunchKernelGGL((adapter_rows<T, RT, VecX, VecB, VecY>), dim3(unsigned(tiles * columns)),
+                       dim3(kAdapterThreads), 0, s, a, columns, width);
 }
 
 template <class T, int RT>
-void launch_rank(const AdapterArgs &a, const AdapterPlan &p, hipStream_t s) {
+void launch_rank(const AdapterArgs &a, hipStream_t s) {
     auto at16 = [](const void *q) { return reinterpret_cast<uintptr_t>(q) % 16 == 0; };
     const bool x = a.ldx % 8 == 0 && at16(a.x), b = a.rank % 8 == 0;
     const bool y = a.ldy % 8 == 0 && at16(a.y) && at16(a.base);
     // (Ranks that are no multiple of 8, and rows off 16-byte boundaries, load by element.)
-    if (x && b && y) launch_as<T, RT, true, true, true>(a, p, s);
-    else if (x && y) launch_as<T, RT, true, false, true>(a, p, s);
-    else if (b) launch_as<T, RT, false, true, false>(a, p, s);
-    else launch_as<T, RT, false, false, false>(a, p, s);
+    if (x && b && y) launch_as<T, RT, true, true, true>(a, s);
+    else if (x && y) launch_as<T, RT, true, false, true>(a, s);
+    else if (b) launch_as<T, RT, false, true, false>(a, s);
+    else launch_as<T, RT, false, false, false>(a, s);
 }
 
-template <class T> void launch_type(const AdapterArgs &a, const AdapterPlan &p, hipStream_t s) {
-    if (a.rank <= 16) launch_rank<T, 1>(a, p, s);
-    else if (a.rank <= 32) launch_rank<T, 2>(a, p, s);
-    else if (a.rank <= 64) launch_rank<T, 4>(a, p, s);
-    else launch_rank<T, 8>(a, p, s);
+template <class T> void launch_type(const AdapterArgs &a, hipStream_t s) {
+    if (a.rank <= 16) launch_rank<T, 1>(a, s);
+    else if (a.rank <= 32) launch_rank<T, 2>(a, s);
+    else if (a.rank <= 64) launch_rank<T, 4>(a, s);
+    else launch_rank<T, 8>(a, s);
 }
 
 }  // namespace
 
-size_t adapter_workspace_bytes(int rows, int adapters, int N, int K, int rank) {
-    const AdapterPlan p = plan_adapter(rows, adapters, N, K, rank);
-    const int pad = rank <= 32 ? 32 : rank <= 64 ? 64 : 128;
-    return size_t(p.splits) * rows * pad * 4;
-}
-
 void launch_adapter(const AdapterArgs &a, hipStream_t s) {
-    const AdapterPlan p = plan_adapter(a.rows, a.adapters, a.N, a.K, a.rank);
-    if (a.type == F16) launch_type<f16_t>(a, p, s);
-    else launch_type<bf16_t>(a, p, s);
+    if (a.type == F16) launch_type<f16_t>(a, s);
+    else launch_type<bf16_t>(a, s);
 }
 
 }  // namespace qlin

@@ -58,16 +58,43 @@ int check_grouping(const char *what, const int *ids, long count, int groups, con
     return QLIN_OK;
 }
 
-// The macro tile for `slots` rows in `experts` groups.
-int choose_tile(long slots, int experts, int N, int K, int fmt, int group) {
-    (void)N;
-    (void)K;
-    (void)fmt;
-    const long each = slots / experts;  // rows per expert, if they are even
-    if (each <= 16) return 1;
-    if (each <= 48) return 4;
-    if (group || each <= 192) return 5;
-    return 7;
+// The macro tile (index of kExpertTiles) for `slots` rows in `experts` groups,
+// of whose sizes the host knows no more than their mean. Measured with uneven
+// groups (weights from HBM, 80 shapes of 8-64 experts, 1024-4096 channels, K
+// 1024-4096, 0.25-1024 rows per expert, INT8 and group FP8):
+//  - up to 8 rows per expert the weights' bytes are all: 64x32 tiles, two or three
+//    workgroups per CU (32 experts of 2048 x 2048, 4 rows each: 25 us, 28 with the
+//    K-sliced 32x16 tile). Where they would leave CUs without work, the K-sliced
+//    tile has twice the workgroups, each a quarter of the K walk (16 of 1024 x
+//    4096, 1 row: 11.2 us against 16.3; 8 of 64, 2048 x 2048: 8.5 against 9.3; with K
+//    groups only from K above 2048: 11.9 against 10.3 at 2048);
+//  - up to 96 rows 128x64 (16 rows: 27.8 us against 31.7 on 64x32, 31.5 on 128x128),
+//    but 64x32 up to 32 rows where 128-channel tiles leave CUs without work (16 of
+//    1024 x 4096, 16 rows: 21.2 against 24.1);
+//  - above, the tile whose rounds of workgroups cost least, at the time that a
+//    workgroup takes per 128 of K when every CU has its share (128x64: two per CU).
+//    Within 8% of the best tile on the shapes above but for one (10%).
+int choose_tile(long slots, int experts, int N, int K, int group) {
+    const long each = slots / experts;
+    const long some = slots < experts ? slots : experts;  // groups that can have rows
+    if (each <= 8)
+        return some * ((N + 63) / 64) <= 256 && (!group || K > 2048) ? 0 : 1;
+    if (each <= 32 && some * ((N + 127) / 128) < 256) return 1;
+    if (each <= 96) return 2;
+    constexpr struct { int tile, per_round, ns, ns_grouped; } kCost[] = {
+        {2, 512, 850, 1180}, {3, 256, 640, 1110}, {4, 256, 1190, 0}, {5, 256, 2060, 0}};
+    int best = 2;
+    long least = LONG_MAX;
+    for (const auto &c : kCost) {
+        const auto &t = qlin::kExpertTiles[c.tile];
+        if (group && !c.ns_grouped) continue;
+        // A group's last tile is short: on average 0.6 of a tile more, at least one.
+        const long rows = slots / t.tokens + experts * 3L / 5;
+        const long tiles = (rows > experts ? rows : experts) * ((N + t.channels - 1) / t.channels);
+        const long cost = (tiles + c.per_round - 1) / c.per_round * (group ? c.ns_grouped : c.ns);
+        if (cost < least) least = cost, best = c.tile;
+    }
+    return best;
 }
 
 int tile_index(const qlin_path &p) {
@@ -165,7 +192,7 @@ int qlin_expert_plan(int slots, int experts, int N, int K, int fmt, int group, q
     if (!path) return fail(QLIN_ERR_INVALID, "path is null");
     const int status = check_expert_shape(slots, experts, N, K, fmt, group);
     if (status) return status;
-    const auto &t = qlin::kExpertTiles[choose_tile(slots, experts, N, K, fmt, group)];
+    const auto &t = qlin::kExpertTiles[choose_tile(slots, experts, N, K, group)];
     *path = {t.slices > 1 ? QLIN_KIND_SKINNY : QLIN_KIND_TILED, t.tokens, t.channels, 1, t.waves, 0};
     return qlin::set_error(QLIN_OK, "");
 }
@@ -198,12 +225,15 @@ int qlin_expert_gemm(const qlin_path *path, const void *x, const float *sx, int 
     // So are the K groups' scales, the tokens' and one expert's.
     if (group && (long(K) + 127) / 128 * (N > x_rows ? N : x_rows) * 4 > INT32_MAX)
         return fail(QLIN_ERR_UNSUPPORTED, "K-group scale arrays exceed 2 GiB");
-    int tile = choose_tile(slots, experts, N, K, fmt, group);
+    int tile = choose_tile(slots, experts, N, K, group);
     if (path && path->kind) {
         tile = path->splits == 1 && path->staged == 0 ? tile_index(*path) : -1;
         if (tile < 0)
             return fail(QLIN_ERR_UNSUPPORTED, "no grouped %dx%d path of %d waves (kind %d)",
                         path->channels, path->tokens, path->waves, path->kind);
+        if (group && tile >= qlin::kExpertNarrowTiles)
+            return fail(QLIN_ERR_UNSUPPORTED, "grouped %dx%d path has per-channel scales only",
+                        path->channels, path->tokens);
     }
     const auto &t = qlin::kExpertTiles[tile];
     if (long(t.channels > t.tokens ? t.channels : t.tokens) * K > INT32_MAX)
@@ -219,15 +249,10 @@ int qlin_expert_gemm(const qlin_path *path, const void *x, const float *sx, int 
     return check_launch("grouped GEMM launch");
 }
 
-size_t qlin_adapter_workspace_bytes(int rows, int adapters, int N, int K, int rank) {
-    if (rows < 1 || adapters < 1 || N < 1 || K < 1 || rank < 1) return 0;
-    return qlin::adapter_workspace_bytes(rows, adapters, N, K, rank);
-}
-
 int qlin_adapter_add(const void *x, int ldx, const int *order, const int *offsets, int rows,
                      int adapters, const void *a, const void *b, int rank, const int *ranks,
                      const float *scales, const void *base, void *y, int ldy, int N, int K, int type,
-                     void *workspace, size_t workspace_bytes, qlin_stream_t stream) {
+                     qlin_stream_t stream) {
     if (type != QLIN_BF16 && type != QLIN_F16)
         return fail(QLIN_ERR_INVALID, "adapter type must be BF16 or F16");
     if (rows < 1 || rows > kMaxIds || N < 1 || K < 1 || K % 16 || N % 16 || ldx < K || ldy < N)
@@ -250,14 +275,10 @@ int qlin_adapter_add(const void *x, int ldx, const int *order, const int *offset
         return fail(QLIN_ERR_INVALID, "adapter output overlaps its input");
     if (base && base != y && overlap(base, y_bytes, y, y_bytes))
         return fail(QLIN_ERR_INVALID, "adapter output overlaps part of its base");
-    const size_t need = qlin::adapter_workspace_bytes(rows, adapters, N, K, rank);
-    if (need && (!workspace || workspace_bytes < need))
-        return fail(QLIN_ERR_WORKSPACE, "adapter workspace of %zu bytes needed, %zu given", need,
-                    workspace ? workspace_bytes : size_t(0));
-    if (need && !aligned(workspace, 16))
-        return fail(QLIN_ERR_ALIGNMENT, "workspace must be 16-byte aligned");
+    if (qlin::expert_row_tiles(rows, adapters, 16) * ((long(N) + 255) / 256) > INT32_MAX)
+        return fail(QLIN_ERR_UNSUPPORTED, "adapter call has more than 2^31 - 1 tiles");
     qlin::launch_adapter({x, order, offsets, a, b, ranks, scales, base, y, ldx, ldy, rows, adapters,
-                          rank, N, K, type, workspace},
+                          rank, N, K, type},
                          reinterpret_cast<hipStream_t>(stream));
     return check_launch("adapter launch");
 }

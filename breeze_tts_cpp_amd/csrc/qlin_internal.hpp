@@ -188,31 +188,25 @@ struct ExpertArgs {
     int x_rows, divisor, scatter, experts, slots, N, K, fmt, out_type, group;
 };
 // Macro tiles: index, K slices, waves along channels and tokens, 16-row
-// fragments per wave of both, LDS stages, waves per SIMD.
-#define QLIN_EXPERT_TILES(X)   \
-    X(0, 1, 2, 1, 4, 1, 3, 2)  \
-    X(1, 1, 2, 1, 2, 1, 4, 2)  \
-    X(2, 4, 1, 1, 2, 1, 3, 2)  \
-    X(3, 4, 1, 1, 4, 1, 3, 1)  \
-    X(4, 1, 4, 1, 2, 2, 2, 4)  \
-    X(5, 2, 2, 2, 2, 2, 2, 4)  \
-    X(6, 1, 2, 4, 4, 2, 2, 4)  \
-    X(7, 1, 4, 2, 4, 4, 3, 2)  \
-    X(8, 1, 2, 2, 2, 2, 2, 4)  \
-    X(9, 1, 4, 1, 1, 2, 3, 4)  \
-    X(10, 1, 4, 2, 2, 2, 3, 4) \
-    X(11, 2, 2, 1, 2, 1, 3, 2) \
-    X(12, 1, 4, 2, 2, 2, 2, 4) \
-    X(13, 1, 2, 4, 8, 4, 2, 2) \
-    X(14, 1, 4, 1, 2, 4, 2, 3) \
-    X(15, 1, 4, 1, 2, 2, 3, 3) \
-    X(16, 1, 2, 4, 4, 2, 3, 2)
+// fragments per wave of both, LDS stages, waves per SIMD. The wide ones have no
+// K-group variant: their accumulators leave no registers for a group's partial
+// sums (a 256x128 tile spills and takes 1.2-1.6 times the 128x64 tile's time).
+#define QLIN_EXPERT_TILES(X)  \
+    X(0, 4, 1, 1, 2, 1, 3, 2) \
+    X(1, 1, 4, 1, 1, 2, 3, 4) \
+    X(2, 1, 4, 2, 2, 2, 3, 4) \
+    X(3, 1, 2, 4, 4, 2, 3, 2)
+#define QLIN_EXPERT_WIDE_TILES(X) \
+    X(4, 1, 4, 2, 4, 4, 3, 2)     \
+    X(5, 1, 2, 4, 8, 4, 2, 2)
+constexpr int kExpertNarrowTiles = 4;
 struct ExpertTile {
     int channels, tokens, waves, slices;
 };
 #define QLIN_EXPERT_TILE(I, KS, WN, WM, NF, MT, S, EU) \
     ExpertTile{16 * (NF) * (WN), 16 * (MT) * (WM), (KS) * (WN) * (WM), KS},
-constexpr ExpertTile kExpertTiles[] = {QLIN_EXPERT_TILES(QLIN_EXPERT_TILE)};
+constexpr ExpertTile kExpertTiles[] = {QLIN_EXPERT_TILES(QLIN_EXPERT_TILE)
+                                       QLIN_EXPERT_WIDE_TILES(QLIN_EXPERT_TILE)};
 #undef QLIN_EXPERT_TILE
 // Most row tiles that `slots` rows in `groups` groups can make.
 constexpr long expert_row_tiles(long slots, long groups, long height) {
@@ -232,9 +226,7 @@ struct AdapterArgs {
     const void *base;    // [rows, ldy] or null
     void *y;             // [rows, ldy]
     int ldx, ldy, rows, adapters, rank, N, K, type;
-    void *workspace;     // adapter_workspace_bytes
 };
-size_t adapter_workspace_bytes(int rows, int adapters, int N, int K, int rank);
 void launch_adapter(const AdapterArgs &, hipStream_t);
 
 // Records `message` as qlin_last_error() of this thread; returns status.

@@ -76,8 +76,7 @@ EXPORTS = ("qlin_version", "qlin_last_error", "qlin_row_quantize", "qlin_plan",
            "qlin_norm_fusion_init", "qlin_epilogue_init", "qlin_layer_norm_quantize",
            "qlin_pointwise_quantize", "qlin_pointwise", "qlin_linear_noalloc", "qlin_noalloc_scratch_bytes",
            "qlin_group_rows_workspace_bytes", "qlin_group_rows", "qlin_route", "qlin_combine",
-           "qlin_expert_plan", "qlin_expert_gemm", "qlin_adapter_workspace_bytes",
-           "qlin_adapter_add")
+           "qlin_expert_plan", "qlin_expert_gemm", "qlin_adapter_add")
 
 
 def load():
@@ -151,10 +150,8 @@ def load():
     L.qlin_expert_gemm.restype = i
     L.qlin_expert_gemm.argtypes = [ctypes.POINTER(qlin_path), P, P, i, P, i, P, P, P, i, P, i, i, i,
                                    i, i, i, i, P]
-    L.qlin_adapter_workspace_bytes.restype = sz
-    L.qlin_adapter_workspace_bytes.argtypes = [i, i, i, i, i]
     L.qlin_adapter_add.restype = i
-    L.qlin_adapter_add.argtypes = [P, i, P, P, i, i, P, P, i, P, P, P, P, i, i, i, i, P, sz, P]
+    L.qlin_adapter_add.argtypes = [P, i, P, P, i, i, P, P, i, P, P, P, P, i, i, i, i, P]
     _lib = L
     return L
 
@@ -166,7 +163,8 @@ def _check(status: int):
 
 def _stream(stream) -> int:
     if stream is None:
-        stream = torch.cuda.current_stream()
+        # The handle alone: building the Stream object takes 2.7 us of a call's 10.
+        return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
     return stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream)
 
 
@@ -545,31 +543,52 @@ def linear_noalloc(x: torch.Tensor, wq: torch.Tensor, sw: torch.Tensor, fmt: int
 
 
 # ---------------------------------------------------------------- rows grouped by weights
+# These run between the products of a decode step, where a call's time on the
+# host is what counts (a launch alone is about 4 us of it): checks read plain
+# tensor attributes, and buffers are made in their final shape.
 _LOGITS = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
+_int32 = torch.int32
+_current_device = torch.cuda.current_device
+
+
+def _on_device(first: torch.Tensor, *others) -> int:
+    """The device of all the tensors given: the current one, on whose stream
+    the call runs."""
+    device = first.get_device()
+    if device < 0 or device != _current_device():
+        raise ValueError("operands must be on the current GPU")
+    for t in others:
+        if t is not None and t.get_device() != device:
+            raise ValueError("operands must be on one GPU, the current one")
+    return device
 
 
 def _indices(t, name, count=None):
-    if t.dtype != torch.int32 or not t.is_contiguous() or (count is not None and t.numel() != count):
+    if t.dtype != _int32 or not t.is_contiguous() or (count is not None and t.numel() != count):
         raise ValueError(f"{name} must be a dense int32 tensor"
                          + ("" if count is None else f" of {count} values"))
     return t
 
 
-def _group_buffers(count, groups, device, order, slots, offsets, workspace):
-    new = lambda n: torch.empty(n, dtype=torch.int32, device=device)
-    order = new(count) if order is None else _indices(order, "order", count)
-    slots = new(count) if slots is None else _indices(slots, "slots", count)
-    offsets = new(groups + 1) if offsets is None else _indices(offsets, "offsets", groups + 1)
-    need = int(load().qlin_group_rows_workspace_bytes(count, groups))
-    if need and workspace is None:
-        workspace = torch.empty(need, dtype=torch.uint8, device=device)
-    return order, slots, offsets, workspace
+def _floats(t, name, count):
+    if t.dtype != torch.float32 or not t.is_contiguous() or t.numel() != count:
+        raise ValueError(f"{name} must be a dense f32 tensor of {count} values")
+    return t
 
 
-def _workspace_args(workspace):
-    if workspace is None:
-        return None, 0
-    return workspace.data_ptr(), workspace.numel() * workspace.element_size()
+def _buffer(workspace, need, device, stream):
+    """(tensor to keep alive, pointer, bytes) of a workspace of `need` bytes. One
+    made here is the allocator's again once the call returns: a stream other
+    than the current one has to be known to it."""
+    if workspace is not None:
+        return workspace, workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    if not need:
+        return None, None, 0
+    workspace = torch.empty(need, dtype=torch.uint8, device=device)
+    if stream is not None:
+        workspace.record_stream(stream if isinstance(stream, torch.cuda.Stream)
+                                else torch.cuda.ExternalStream(_stream(stream), device=device))
+    return workspace, workspace.data_ptr(), need
 
 
 def group_rows(ids: torch.Tensor, groups: int, order=None, slots=None, offsets=None,
@@ -577,13 +596,20 @@ def group_rows(ids: torch.Tensor, groups: int, order=None, slots=None, offsets=N
     """Rows grouped by id (qlin_group_rows): int32 ids of any shape, those
     outside [0, groups) in no group. Returns (order, slots, offsets); slots has
     the shape of ids."""
+    L = _lib or load()
     _indices(ids, "ids")
-    order, slots, offsets, workspace = _group_buffers(ids.numel(), groups, ids.device, order, slots,
-                                                      offsets, workspace)
-    _check(load().qlin_group_rows(ids.data_ptr(), ids.numel(), groups, order.data_ptr(),
-                                  slots.data_ptr(), offsets.data_ptr(), *_workspace_args(workspace),
-                                  _stream(stream)))
-    return order, slots.view(ids.shape), offsets
+    count = ids.numel()
+    order = torch.empty(count, dtype=_int32, device=ids.device) if order is None \
+        else _indices(order, "order", count)
+    slots = torch.empty_like(ids) if slots is None else _indices(slots, "slots", count)
+    offsets = torch.empty(groups + 1, dtype=_int32, device=ids.device) if offsets is None \
+        else _indices(offsets, "offsets", groups + 1)
+    need = L.qlin_group_rows_workspace_bytes(count, groups) if count > 4096 else 0
+    workspace, ws_ptr, ws_bytes = _buffer(workspace, need, ids.device, stream)
+    _on_device(ids, order, slots, offsets, workspace)
+    _check(L.qlin_group_rows(ids.data_ptr(), count, groups, order.data_ptr(), slots.data_ptr(),
+                             offsets.data_ptr(), ws_ptr, ws_bytes, _stream(stream)))
+    return order, slots if slots.shape == ids.shape else slots.view(ids.shape), offsets
 
 
 def route(logits: torch.Tensor, top_k: int, normalize: bool = False, ids=None, weights=None,
@@ -591,25 +617,34 @@ def route(logits: torch.Tensor, top_k: int, normalize: bool = False, ids=None, w
     """Router (qlin_route): f32/bf16/f16 logits [tokens, experts] (row stride
     allowed) -> ids int32 [tokens, top_k], weights f32 [tokens, top_k], and the
     choices grouped by expert: order, slots [tokens, top_k], offsets."""
-    if logits.dim() != 2 or logits.stride(1) != 1 or logits.dtype not in _LOGITS:
+    L = _lib or load()
+    kind = _LOGITS.get(logits.dtype)
+    if kind is None or logits.dim() != 2:
         raise ValueError("route expects 2-D f32/bf16/f16 logits with unit column stride")
     tokens, experts = logits.shape
-    ld = logits.stride(0) if tokens > 1 else experts
-    count = tokens * top_k
-    if ids is None:
-        ids = torch.empty((tokens, top_k), dtype=torch.int32, device=logits.device)
-    if weights is None:
-        weights = torch.empty((tokens, top_k), dtype=torch.float32, device=logits.device)
-    _indices(ids, "ids", count)
-    if weights.dtype != torch.float32 or not weights.is_contiguous() or weights.numel() != count:
-        raise ValueError(f"weights must be a dense f32 tensor of {count} values")
-    order, slots, offsets, workspace = _group_buffers(count, experts, logits.device, order, slots,
-                                                      offsets, workspace)
-    _check(load().qlin_route(logits.data_ptr(), ld, _LOGITS[logits.dtype], tokens, experts, top_k,
-                             int(normalize), ids.data_ptr(), weights.data_ptr(), order.data_ptr(),
-                             slots.data_ptr(), offsets.data_ptr(), *_workspace_args(workspace),
-                             _stream(stream)))
-    return ids, weights, order, slots.view(tokens, top_k), offsets
+    ld, unit = logits.stride()
+    if unit != 1 and experts > 1:
+        raise ValueError("route expects 2-D f32/bf16/f16 logits with unit column stride")
+    if tokens == 1 and ld < experts:
+        ld = experts
+    count, device = tokens * top_k, logits.device
+    ids = torch.empty((tokens, top_k), dtype=_int32, device=device) if ids is None \
+        else _indices(ids, "ids", count)
+    weights = torch.empty((tokens, top_k), dtype=torch.float32, device=device) \
+        if weights is None else _floats(weights, "weights", count)
+    order = torch.empty(count, dtype=_int32, device=device) if order is None \
+        else _indices(order, "order", count)
+    slots = torch.empty((tokens, top_k), dtype=_int32, device=device) if slots is None \
+        else _indices(slots, "slots", count).view(tokens, top_k)
+    offsets = torch.empty(experts + 1, dtype=_int32, device=device) if offsets is None \
+        else _indices(offsets, "offsets", experts + 1)
+    need = L.qlin_group_rows_workspace_bytes(count, experts) if count > 4096 else 0
+    workspace, ws_ptr, ws_bytes = _buffer(workspace, need, device, stream)
+    _on_device(logits, ids, weights, order, slots, offsets, workspace)
+    _check(L.qlin_route(logits.data_ptr(), ld, kind, tokens, experts, top_k, normalize,
+                        ids.data_ptr(), weights.data_ptr(), order.data_ptr(), slots.data_ptr(),
+                        offsets.data_ptr(), ws_ptr, ws_bytes, _stream(stream)))
+    return ids, weights, order, slots, offsets
 
 
 def combine(h: torch.Tensor, slots: torch.Tensor, weights: torch.Tensor | None = None,
@@ -617,24 +652,26 @@ def combine(h: torch.Tensor, slots: torch.Tensor, weights: torch.Tensor | None =
     """The experts' rows back to their tokens (qlin_combine): h [rows, N],
     slots int32 [tokens, top_k], weights f32 of the same shape (None = 1),
     base [tokens, N] or None. out may be base. Returns out [tokens, N]."""
-    if h.dim() != 2 or not h.is_contiguous() or h.dtype not in _TYPES:
+    L = _lib or load()
+    kind = _TYPES.get(h.dtype)
+    if kind is None or h.dim() != 2 or not h.is_contiguous():
         raise ValueError("combine expects dense 2-D bf16/f16 rows")
     if slots.dim() != 2:
         raise ValueError("combine expects slots [tokens, top_k]")
     _indices(slots, "slots")
     tokens, top_k = slots.shape
-    if weights is not None and (weights.dtype != torch.float32 or not weights.is_contiguous()
-                                or weights.shape != slots.shape):
-        raise ValueError("combine weights must be dense f32 in the shape of slots")
+    h_rows, N = h.shape
+    if weights is not None:
+        _floats(weights, "weights", tokens * top_k)
     if out is None:
-        out = torch.empty((tokens, h.shape[1]), dtype=h.dtype, device=h.device)
+        out = torch.empty((tokens, N), dtype=h.dtype, device=h.device)
     for t in (base, out):
-        if t is not None and (t.shape != (tokens, h.shape[1]) or t.dtype != h.dtype
+        if t is not None and (t.shape != (tokens, N) or t.dtype != h.dtype
                               or not t.is_contiguous()):
             raise ValueError("combine base and output must be dense [tokens, N] in the rows' type")
-    _check(load().qlin_combine(h.data_ptr(), h.shape[0], slots.data_ptr(), _ptr(weights), _ptr(base),
-                               out.data_ptr(), tokens, top_k, h.shape[1], _TYPES[h.dtype],
-                               _stream(stream)))
+    _on_device(h, slots, weights, base, out)
+    _check(L.qlin_combine(h.data_ptr(), h_rows, slots.data_ptr(), _ptr(weights), _ptr(base),
+                          out.data_ptr(), tokens, top_k, N, kind, _stream(stream)))
     return out
 
 
@@ -653,71 +690,66 @@ def expert_gemm(xq: torch.Tensor, sx: torch.Tensor, wq: torch.Tensor, sw: torch.
     [experts, ceil(K/128), N]; sx [ceil(K/128), x_rows]). With `order` slot s
     reads row order[s] // divisor (and with `scatter` writes row order[s]), else
     row s. Returns out [slots, N]; rows of no group keep what out held."""
+    L = _lib or load()
     if xq.dim() != 2 or wq.dim() != 3 or xq.shape[1] != wq.shape[2]:
         raise ValueError("expert_gemm expects codes [x_rows, K] and weights [experts, N, K]")
-    if not (xq.is_contiguous() and wq.is_contiguous() and sx.is_contiguous() and sw.is_contiguous()):
-        raise ValueError("expert_gemm operands must be dense")
-    if xq.element_size() != 1 or wq.element_size() != 1:
-        raise ValueError("expert_gemm operands must be 8-bit codes")
+    if xq.element_size() != 1 or wq.element_size() != 1 or not xq.is_contiguous() \
+            or not wq.is_contiguous():
+        raise ValueError("expert_gemm operands must be dense 8-bit codes")
     x_rows, K = xq.shape
     experts, N, _ = wq.shape
-    blocks = (K + group - 1) // group if group else 1
-    if sx.dtype != torch.float32 or sw.dtype != torch.float32 or sx.numel() != blocks * x_rows \
-            or sw.numel() != experts * blocks * N:
-        raise ValueError("expert_gemm scales must be f32, one per row or per row and K group")
+    blocks = (K + group - 1) // group if group > 0 else 1
+    _floats(sx, "expert_gemm row scales", blocks * x_rows)
+    _floats(sw, "expert_gemm channel scales", experts * blocks * N)
     _indices(offsets, "offsets", experts + 1)
     slots = x_rows if order is None else _indices(order, "order").numel()
     if out is None:
         out = torch.empty((slots, N), dtype=out_dtype, device=xq.device)
-    if out.shape != (slots, N) or out.dtype not in _TYPES or not out.is_contiguous():
+    kind = _TYPES.get(out.dtype)
+    if kind is None or out.shape != (slots, N) or not out.is_contiguous():
         raise ValueError("expert_gemm output must be dense bf16/f16 [slots, N]")
-    p = (path or Path()).to_c()
-    _check(load().qlin_expert_gemm(ctypes.byref(p), xq.data_ptr(), sx.data_ptr(), x_rows, _ptr(order),
-                                   divisor, offsets.data_ptr(), wq.data_ptr(), sw.data_ptr(), experts,
-                                   out.data_ptr(), int(scatter), slots, N, K, fmt, _TYPES[out.dtype],
-                                   group, _stream(stream)))
+    _on_device(xq, sx, wq, sw, offsets, order, out)
+    _check(L.qlin_expert_gemm(None if path is None else ctypes.byref(path.to_c()), xq.data_ptr(),
+                              sx.data_ptr(), x_rows, _ptr(order), divisor, offsets.data_ptr(),
+                              wq.data_ptr(), sw.data_ptr(), experts, out.data_ptr(), scatter, slots,
+                              N, K, fmt, kind, group, _stream(stream)))
     return out
-
-
-def adapter_workspace_bytes(rows: int, adapters: int, N: int, K: int, rank: int) -> int:
-    return int(load().qlin_adapter_workspace_bytes(rows, adapters, N, K, rank))
 
 
 def adapter_add(x: torch.Tensor, order: torch.Tensor, offsets: torch.Tensor, a: torch.Tensor,
                 b: torch.Tensor, y: torch.Tensor, base: torch.Tensor | None = None,
-                ranks: torch.Tensor | None = None, scales: torch.Tensor | None = None,
-                workspace: torch.Tensor | None = None, stream=None):
+                ranks: torch.Tensor | None = None, scales: torch.Tensor | None = None, stream=None):
     """Low-rank adapters beside a shared projection (qlin_adapter_add): rows of
     adapter g get y = base + scales[g] * (x a[g]^T) b[g]^T in x's 16-bit type;
     a [adapters, rank, K], b [adapters, N, rank], order / offsets of
     group_rows(ids, adapters). base None: y itself (the projection's output).
     x and y may be column ranges of wider rows. Returns y."""
-    if x.dim() != 2 or x.stride(1) != 1 or x.dtype not in _TYPES:
+    L = _lib or load()
+    dtype = x.dtype
+    kind = _TYPES.get(dtype)
+    if kind is None or x.dim() != 2 or (x.stride(1) != 1 and x.shape[1] > 1):
         raise ValueError("adapter_add expects 2-D bf16/f16 rows with unit column stride")
-    if a.dim() != 3 or b.dim() != 3 or a.shape[0] != b.shape[0] or a.shape[1] != b.shape[2] \
-            or a.shape[2] != x.shape[1] or not (a.is_contiguous() and b.is_contiguous()) \
-            or a.dtype != x.dtype or b.dtype != x.dtype:
-        raise ValueError("adapter_add expects dense a [adapters, rank, K] and b [adapters, N, rank]")
     rows, K = x.shape
+    if b.dim() != 3:
+        raise ValueError("adapter_add expects dense a [adapters, rank, K] and b [adapters, N, rank]")
     adapters, N, rank = b.shape
+    if a.shape != (adapters, rank, K) or a.dtype != dtype or b.dtype != dtype \
+            or not a.is_contiguous() or not b.is_contiguous():
+        raise ValueError("adapter_add expects dense a [adapters, rank, K] and b [adapters, N, rank]")
     _indices(order, "order", rows)
     _indices(offsets, "offsets", adapters + 1)
     base = y if base is None else base
+    ldx, ldy = (x.stride(0), y.stride(0)) if rows > 1 else (K, N)
     for t in (y, base):
-        if t.shape != (rows, N) or t.dtype != x.dtype or t.stride(1) != 1 \
-                or (rows > 1 and t.stride(0) != y.stride(0)):
+        if t.shape != (rows, N) or t.dtype != dtype or (t.stride(1) != 1 and N > 1) \
+                or (rows > 1 and t.stride(0) != ldy):
             raise ValueError("adapter_add base and output must be [rows, N] rows of one stride")
     if ranks is not None:
         _indices(ranks, "ranks", adapters)
-    if scales is not None and (scales.dtype != torch.float32 or not scales.is_contiguous()
-                               or scales.numel() != adapters):
-        raise ValueError("adapter_add scales must be dense f32 [adapters]")
-    need = adapter_workspace_bytes(rows, adapters, N, K, rank)
-    if need and workspace is None:
-        workspace = torch.empty(need, dtype=torch.uint8, device=x.device)
-    ldx, ldy = (x.stride(0), y.stride(0)) if rows > 1 else (K, N)
-    _check(load().qlin_adapter_add(x.data_ptr(), ldx, order.data_ptr(), offsets.data_ptr(), rows,
-                                   adapters, a.data_ptr(), b.data_ptr(), rank, _ptr(ranks),
-                                   _ptr(scales), base.data_ptr(), y.data_ptr(), ldy, N, K,
-                                   _TYPES[x.dtype], *_workspace_args(workspace), _stream(stream)))
+    if scales is not None:
+        _floats(scales, "scales", adapters)
+    _on_device(x, order, offsets, a, b, y, base, ranks, scales)
+    _check(L.qlin_adapter_add(x.data_ptr(), ldx, order.data_ptr(), offsets.data_ptr(), rows, adapters,
+                              a.data_ptr(), b.data_ptr(), rank, _ptr(ranks), _ptr(scales),
+                              base.data_ptr(), y.data_ptr(), ldy, N, K, kind, _stream(stream)))
     return y

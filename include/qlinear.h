@@ -33,7 +33,7 @@
  *                          scratch in a fixed library-owned device array, for callers
  *                          that cannot allocate
  *   qlin_route, qlin_group_rows, qlin_combine, qlin_expert_gemm, qlin_expert_plan,
- *   qlin_adapter_add and their workspace sizes
+ *   qlin_adapter_add, qlin_group_rows_workspace_bytes
  *                       <- no counterpart in the reference: rows that each name the
  *                          weights they use (experts, codebook heads, adapters)
  *
@@ -430,11 +430,10 @@ int qlin_expert_gemm(const qlin_path *path, const void *x, const float *sx, int 
  * or more. rank <= 128, K % 16 == 0, N % 16 == 0; order names a row at most once.
  * A column range of y (one projection of a merged output) is a y offset by its
  * first column with the whole row's ldy. */
-size_t qlin_adapter_workspace_bytes(int rows, int adapters, int N, int K, int rank);
 int qlin_adapter_add(const void *x, int ldx, const int *order, const int *offsets, int rows,
                      int adapters, const void *a, const void *b, int rank, const int *ranks,
                      const float *scales, const void *base, void *y, int ldy, int N, int K, int type,
-                     void *workspace, size_t workspace_bytes, qlin_stream_t stream);
+                     qlin_stream_t stream);
 
 #ifdef __cplusplus
 }

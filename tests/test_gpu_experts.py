@@ -71,12 +71,14 @@ def every_path():
     from breeze_tts_cpp_amd import qlinear
     seen = []
     for slots in (1, 64, 200, 2000, 6400, 12800, 20000, 40000, 100000):
-        for K in (256, 2048, 6144):
+        for K in (256, 2048, 4096):
             for mode, (fmt, group) in MODES.items():
-                for N in (256, 2048, 12288):
-                    p = qlinear.expert_plan(slots, 64, N, K, fmt, group)
-                    if (mode, p) not in seen:
-                        seen.append((mode, p))
+                for N in (256, 1024, 2048, 4096):
+                    for experts in (8, 64):
+                        p = qlinear.expert_plan(slots, experts, N, K, fmt, group)
+                        if (mode, p) not in seen:
+                            seen.append((mode, p))
+    assert len(seen) == 20  # six tiles per channel, four with K groups
     return seen
 
 

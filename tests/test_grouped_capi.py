@@ -93,6 +93,9 @@ def test_expert_refusals():
     good = qlinear.expert_plan(64, 8, 64, 256, I8)
     assert call(path=qlinear.Path(good.kind, good.tokens, good.channels, 2, good.waves)) == -4
     assert call(path=qlinear.Path(good.kind, good.tokens, good.channels, 1, good.waves + 1)) == -4
+    wide = qlinear.expert_plan(1 << 16, 8, 4096, 2048, I8)
+    assert wide.channels == 256
+    assert call(path=wide, group=128) == -4 and b"per-channel" in L.qlin_last_error()
     assert call(slots=1 << 30, order=FAKE, x_rows=1, N=1 << 20, K=16) == -4
     p = qlinear.qlin_path()
     assert L.qlin_expert_plan(64, 8, 64, 256, I8, 0, None) == -1
@@ -103,9 +106,9 @@ def test_adapter_refusals():
     L = qlinear.load()
 
     def call(x=FAKE, ldx=256, order=FAKE, off=FAKE, rows=8, n=4, a=FAKE, b=FAKE, rank=16, ranks=None,
-             scales=None, base=None, y=FAR, ldy=64, N=64, K=256, t=BF16, ws=None, wsb=0):
+             scales=None, base=None, y=FAR, ldy=64, N=64, K=256, t=BF16):
         return L.qlin_adapter_add(x, ldx, order, off, rows, n, a, b, rank, ranks, scales, base, y,
-                                  ldy, N, K, t, ws, wsb, None)
+                                  ldy, N, K, t, None)
 
     assert call(t=F32) == -1 and call(rows=0) == -1 and call(N=40) == -1 and call(K=200) == -1
     assert call(ldx=255) == -1 and call(ldy=63) == -1
@@ -117,10 +120,7 @@ def test_adapter_refusals():
     assert call(order=FAKE + 2) == -2 and call(scales=FAKE + 1) == -2 and call(ranks=FAKE + 2) == -2
     assert call(y=FAKE + 64) == -1 and b"overlaps" in L.qlin_last_error()
     assert call(base=FAR + 2) == -1
-    need = L.qlin_adapter_workspace_bytes(4096, 4, 64, 256, 16)
-    assert need > 0
-    assert call(rows=4096) == -3 and call(rows=4096, ws=FAKE, wsb=need - 1) == -3
-    assert call(rows=4096, ws=FAKE + 4, wsb=need) == -2
+    assert call(rows=1 << 30, N=1 << 20, ldy=1 << 20, x=1 << 60) == -4 and b"tiles" in L.qlin_last_error()
 
 
 def test_binding_refusals():
