@@ -72,26 +72,36 @@ int check_grouping(const char *what, const int *ids, long count, int groups, con
 //    but 64x32 up to 32 rows where 128-channel tiles leave CUs without work (16 of
 //    1024 x 4096, 16 rows: 21.2 against 24.1);
 //  - above, the tile whose rounds of workgroups cost least, at the time that a
-//    workgroup takes per 128 of K when every CU has its share (128x64: two per CU).
-//    Within 8% of the best tile on the shapes above but for one (10%).
+//    round of each takes with uneven groups (128x64: two workgroups per CU), a part
+//    per 128 of K and a fixed one (prologue, epilogue).
+// With K groups 128x64 from 4 rows (6 rows, 31 experts of 2064 x 2048: 23.3 us, 26.3 on
+// 64x32). On the 80 shapes the choice is within 6% of the best tile.
 int choose_tile(long slots, int experts, int N, int K, int group) {
     const long each = slots / experts;
     const long some = slots < experts ? slots : experts;  // groups that can have rows
-    if (each <= 8)
-        return some * ((N + 63) / 64) <= 256 && (!group || K > 2048) ? 0 : 1;
+    if (each <= 8 && some * ((N + 63) / 64) <= 256 && (!group || K > 2048)) return 0;
+    if (each <= (group ? 3 : 8)) return 1;
     if (each <= 32 && some * ((N + 127) / 128) < 256) return 1;
     if (each <= 96) return 2;
-    constexpr struct { int tile, per_round, ns, ns_grouped; } kCost[] = {
-        {2, 512, 850, 1180}, {3, 256, 640, 1110}, {4, 256, 1190, 0}, {5, 256, 2060, 0}};
+    constexpr struct { int tile, per_round, stage, fixed, grouped_stage, grouped_fixed; } kCost[] = {
+        {2, 512, 740, 4000, 1020, 2600},
+        {3, 256, 650, 4300, 825, 4500},
+        {4, 256, 975, 7500, 0, 0},
+        {5, 256, 1810, 9900, 0, 0}};  // ns
+    const long stages = (long(K) + 127) / 128;
     int best = 2;
     long least = LONG_MAX;
     for (const auto &c : kCost) {
         const auto &t = qlin::kExpertTiles[c.tile];
-        if (group && !c.ns_grouped) continue;
+        if (group && !c.grouped_stage) continue;
         // A group's last tile is short: on average 0.6 of a tile more, at least one.
         const long rows = slots / t.tokens + experts * 3L / 5;
         const long tiles = (rows > experts ? rows : experts) * ((N + t.channels - 1) / t.channels);
-        const long cost = (tiles + c.per_round - 1) / c.per_round * (group ? c.ns_grouped : c.ns);
+        // Whole rounds while they are few; many even out to half a round more.
+        const long rounds2 = tiles <= 4 * c.per_round ? (tiles + c.per_round - 1) / c.per_round * 2
+                                                      : tiles * 2 / c.per_round + 1;
+        const long cost = rounds2 * (group ? stages * c.grouped_stage + c.grouped_fixed
+                                           : stages * c.stage + c.fixed);
         if (cost < least) least = cost, best = c.tile;
     }
     return best;
@@ -275,6 +285,9 @@ int qlin_adapter_add(const void *x, int ldx, const int *order, const int *offset
         return fail(QLIN_ERR_INVALID, "adapter output overlaps its input");
     if (base && base != y && overlap(base, y_bytes, y, y_bytes))
         return fail(QLIN_ERR_INVALID, "adapter output overlaps part of its base");
+    // Rows of x and an adapter's a are addressed through 32-bit buffer ranges.
+    if (x_bytes > size_t(INT32_MAX) || size_t(rank) * K * 2 > size_t(INT32_MAX))
+        return fail(QLIN_ERR_UNSUPPORTED, "adapter input rows exceed 2 GiB");
     if (qlin::expert_row_tiles(rows, adapters, 16) * ((long(N) + 255) / 256) > INT32_MAX)
         return fail(QLIN_ERR_UNSUPPORTED, "adapter call has more than 2^31 - 1 tiles");
     qlin::launch_adapter({x, order, offsets, a, b, ranks, scales, base, y, ldx, ldy, rows, adapters,

@@ -22,31 +22,38 @@ __device__ __forceinline__ float key_logit(uint32_t k) {
     return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
 
-template <int S> __device__ __forceinline__ uint32_t lane_xor_bits(uint32_t v) {
-    return __float_as_uint(lane_xor<S>(__uint_as_float(v)));
-}
-
-// The larger (key, lower index on ties) of this lane's pair and its partner's.
-template <int S> __device__ __forceinline__ void pick_larger(uint32_t &key, int &at) {
-    const uint32_t k = lane_xor_bits<S>(key);
-    const int a = int(lane_xor_bits<S>(uint32_t(at)));
-    const bool other = k > key || (k == key && a < at);
-    key = other ? k : key;
-    at = other ? a : at;
-}
-
 template <int Type> __device__ __forceinline__ float load_logit(const void *p, size_t i) {
     if constexpr (Type == F32) return static_cast<const float *>(p)[i];
     else if constexpr (Type == F16) return to_float(static_cast<const uint16_t *>(p)[i], f16_t{});
     else return to_float(static_cast<const uint16_t *>(p)[i], bf16_t{});
 }
 
+// f over the lanes' values of an aligned group of L lanes (16 or 64).
+template <int L, class V, class F> __device__ __forceinline__ V across(V v, F f) {
+    auto other = [&](auto s_) {
+        return __builtin_bit_cast(V, lane_xor<decltype(s_)::value>(__builtin_bit_cast(float, v)));
+    };
+    v = f(v, other(std::integral_constant<int, 1>{}));
+    v = f(v, other(std::integral_constant<int, 2>{}));
+    v = f(v, other(std::integral_constant<int, 4>{}));
+    v = f(v, other(std::integral_constant<int, 8>{}));
+    if constexpr (L > 16) {
+        v = f(v, other(std::integral_constant<int, 16>{}));
+        v = f(v, other(std::integral_constant<int, 32>{}));
+    }
+    return v;
+}
+
 // One token by L lanes of a wave (an aligned group), V logits each: expert
-// i * L + l in lane l. Each round takes the largest key left; p = e^(v - max),
-// fp32 sums (normalized: over the chosen in their order; else over all, per
-// lane and then across lanes).
+// i * L + l in lane l. Each round takes the largest key left, the lowest expert
+// of equals. The low 13 bits of a widened 16-bit logit are zero, so its key's low
+// 10 take 1023 - expert and one maximum finds both; fp32 keys need a second pass
+// for the expert.
+// Choice j ends in lane j (top_k <= 16 <= L): p = e^(v - max), the weights' sum in
+// fp32 over the lanes (normalized), or over all logits, per lane first.
 template <int Type, int L, int V>
 __device__ __forceinline__ void route_token(const RouteArgs &a, int token) {
+    constexpr bool kPacked = Type != F32;
     const int l = threadIdx.x % L;
     uint32_t key[V];
 #pragma unroll
@@ -54,56 +61,56 @@ __device__ __forceinline__ void route_token(const RouteArgs &a, int token) {
         const int e = i * L + l;
         const float v = load_logit<Type>(a.logits, size_t(token) * a.ld + min(e, a.experts - 1));
         key[i] = e < a.experts ? logit_key(v) : 0;
+        if (kPacked && key[i]) key[i] = (key[i] & ~0x3ffu) | uint32_t(0x3ff - e);
     }
-    uint32_t top_key = 0;
-    float sum = 0.f, weight = 0.f;  // lane j of the group keeps choice j (top_k <= 16 <= L)
-    int chosen = -1;
+    // The logit of a key as kept.
+    auto value = [&](uint32_t k) {
+        if constexpr (kPacked) k = k & 0x80000000u ? k & ~0x3ffu : k | 0x3ffu;
+        return key_logit(k);
+    };
+    auto larger = [](uint32_t x, uint32_t y) { return x > y ? x : y; };
+    uint32_t mine = 0;
+    int expert = -1;
+    float peak = 0.f, sum = 0.f;
     for (int j = 0; j < a.top_k; ++j) {
-        uint32_t best = 0;
-        int at = 0x7fffffff;
+        uint32_t best = key[0];
 #pragma unroll
-        for (int i = 0; i < V; ++i)
-            if (key[i] > best) best = key[i], at = i * L + l;
-        pick_larger<1>(best, at);
-        pick_larger<2>(best, at);
-        pick_larger<4>(best, at);
-        pick_larger<8>(best, at);
-        if constexpr (L > 16) {
-            pick_larger<16>(best, at);
-            pick_larger<32>(best, at);
-        }
+        for (int i = 1; i < V; ++i) best = larger(best, key[i]);
+        best = across<L>(best, larger);
         if (best == 0) break;  // the same in all L lanes
         if (j == 0) {
-            top_key = best;
+            peak = value(best);
             if (!a.normalize) {
-                const float peak = key_logit(best);
 #pragma unroll
                 for (int i = 0; i < V; ++i)
-                    if (key[i]) sum += key[i] == best ? 1.f : qexp(key_logit(key[i]) - peak);
-                sum += lane_xor<1>(sum);
-                sum += lane_xor<2>(sum);
-                sum += lane_xor<4>(sum);
-                sum += lane_xor<8>(sum);
-                if constexpr (L > 16) {
-                    sum += lane_xor<16>(sum);
-                    sum += lane_xor<32>(sum);
-                }
+                    if (key[i]) sum += value(key[i]) == peak ? 1.f : qexp(value(key[i]) - peak);
             }
         }
-        // (At the maximum itself, +inf too, p is 1; below a maximum of +inf it is 0.)
-        const float p = best == top_key ? 1.f : qexp(key_logit(best) - key_logit(top_key));
-        if (a.normalize) sum += p;
-        if (l == j) weight = p, chosen = at;
+        int at;
+        if constexpr (kPacked) {
+            at = 0x3ff - int(best & 0x3ffu);
+        } else {
+            at = 0x7fffffff;
+#pragma unroll
+            for (int i = V - 1; i >= 0; --i)
+                if (key[i] == best) at = i * L + l;
+            at = across<L>(at, [](int x, int y) { return x < y ? x : y; });
+        }
+        if (l == j) mine = best, expert = at;
 #pragma unroll
         for (int i = 0; i < V; ++i)
             if (i * L + l == at) key[i] = 0;
     }
+    // (At the maximum itself, +inf too, p is 1; below a maximum of +inf it is 0.)
+    const float p = expert < 0 ? 0.f : value(mine) == peak ? 1.f : qexp(value(mine) - peak);
+    sum = across<L>(a.normalize ? p : sum, [](float x, float y) { return x + y; });
     if (l < a.top_k) {
-        a.ids[size_t(token) * a.top_k + l] = chosen;
-        a.weights[size_t(token) * a.top_k + l] = chosen < 0 ? 0.f : weight / sum;
+        a.ids[size_t(token) * a.top_k + l] = expert;
+        a.weights[size_t(token) * a.top_k + l] = expert < 0 ? 0.f : p / sum;
     }
 }
 
+static_assert(kMaxGroups == 1024, "an expert's number in 10 bits");
 constexpr int kRouteThreads = 256;
 template <int Type, int L, int V>
 __global__ __launch_bounds__(kRouteThreads) void route_tokens(RouteArgs a) {
@@ -246,6 +253,7 @@ __global__ __launch_bounds__(kGroupThreads) void group_place(GroupArgs a, int bi
     const int *table = static_cast<const int *>(a.workspace);
     int total = 0, before = 0;
     if (int(threadIdx.x) < a.groups)
+#pragma unroll 8
         for (int b = 0; b < int(gridDim.x); ++b) {
             const int c = table[size_t(b) * a.groups + threadIdx.x];
             before += b < int(blockIdx.x) ? c : 0;

@@ -427,7 +427,8 @@ int qlin_expert_gemm(const qlin_path *path, const void *x, const float *sx, int 
  *   ranks [adapters] or NULL: the ranks in use; the rest of a and b is not used
  *   scales f32 [adapters] or NULL (1)
  * Both products accumulate in fp32 and the inner one is carried with 18 bits
- * or more. rank <= 128, K % 16 == 0, N % 16 == 0; order names a row at most once.
+ * or more. rank <= 128, K % 16 == 0, N % 16 == 0, rows of x within 2 GiB; order names a
+ * row at most once.
  * A column range of y (one projection of a merged output) is a y offset by its
  * first column with the whole row's ldy. */
 int qlin_adapter_add(const void *x, int ldx, const int *order, const int *offsets, int rows,

@@ -120,7 +120,9 @@ def test_adapter_refusals():
     assert call(order=FAKE + 2) == -2 and call(scales=FAKE + 1) == -2 and call(ranks=FAKE + 2) == -2
     assert call(y=FAKE + 64) == -1 and b"overlaps" in L.qlin_last_error()
     assert call(base=FAR + 2) == -1
-    assert call(rows=1 << 30, N=1 << 20, ldy=1 << 20, x=1 << 60) == -4 and b"tiles" in L.qlin_last_error()
+    assert call(rows=1 << 22) == -4 and b"2 GiB" in L.qlin_last_error()
+    assert call(rows=1 << 25, N=1 << 20, ldy=1 << 20, K=16, ldx=16, x=1 << 60) == -4
+    assert b"tiles" in L.qlin_last_error()
 
 
 def test_binding_refusals():
