@@ -259,10 +259,15 @@ int qlin_expert_gemm(const qlin_path *path, const void *x, const float *sx, int 
     return check_launch("grouped GEMM launch");
 }
 
+size_t qlin_adapter_workspace_bytes(int rows, int adapters, int K, int rank) {
+    if (rows < 1 || rows > kMaxIds || adapters < 1 || K < 1 || rank < 1) return 0;
+    return qlin::adapter_workspace_bytes(rows, adapters, K, rank);
+}
+
 int qlin_adapter_add(const void *x, int ldx, const int *order, const int *offsets, int rows,
                      int adapters, const void *a, const void *b, int rank, const int *ranks,
                      const float *scales, const void *base, void *y, int ldy, int N, int K, int type,
-                     qlin_stream_t stream) {
+                     void *workspace, size_t workspace_bytes, qlin_stream_t stream) {
     if (type != QLIN_BF16 && type != QLIN_F16)
         return fail(QLIN_ERR_INVALID, "adapter type must be BF16 or F16");
     if (rows < 1 || rows > kMaxIds || N < 1 || K < 1 || K % 16 || N % 16 || ldx < K || ldy < N)
@@ -285,13 +290,19 @@ int qlin_adapter_add(const void *x, int ldx, const int *order, const int *offset
         return fail(QLIN_ERR_INVALID, "adapter output overlaps its input");
     if (base && base != y && overlap(base, y_bytes, y, y_bytes))
         return fail(QLIN_ERR_INVALID, "adapter output overlaps part of its base");
+    const size_t need = qlin::adapter_workspace_bytes(rows, adapters, K, rank);
+    if (need && (!workspace || workspace_bytes < need))
+        return fail(QLIN_ERR_WORKSPACE, "adapter workspace of %zu bytes needed, %zu given", need,
+                    workspace ? workspace_bytes : size_t(0));
+    if (need && !aligned(workspace, 16))
+        return fail(QLIN_ERR_ALIGNMENT, "workspace must be 16-byte aligned");
     // Rows of x and an adapter's a are addressed through 32-bit buffer ranges.
     if (x_bytes > size_t(INT32_MAX) || size_t(rank) * K * 2 > size_t(INT32_MAX))
         return fail(QLIN_ERR_UNSUPPORTED, "adapter input rows exceed 2 GiB");
     if (qlin::expert_row_tiles(rows, adapters, 16) * ((long(N) + 255) / 256) > INT32_MAX)
         return fail(QLIN_ERR_UNSUPPORTED, "adapter call has more than 2^31 - 1 tiles");
     qlin::launch_adapter({x, order, offsets, a, b, ranks, scales, base, y, ldx, ldy, rows, adapters,
-                          rank, N, K, type},
+                          rank, N, K, type, workspace},
                          reinterpret_cast<hipStream_t>(stream));
     return check_launch("adapter launch");
 }

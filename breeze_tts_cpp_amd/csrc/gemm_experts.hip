@@ -70,13 +70,14 @@ __global__ __launch_bounds__(64 * KS * WN * WM, EU) void expert_gemm(ExpertArgs 
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int row16 = lane & 15, quad = lane >> 4;
     const int ks = wave / NWS, ws = wave % NWS, wn = ws % WN, wm = ws / WN;
-    // The tile's row ml in x, or -1 (past the group, or an order entry outside x).
-    auto source = [&](int ml) {
-        if (ml >= tile.rows) return -1;
-        if (!p.order) return m_base + ml;
-        const int at = p.order[m_base + ml];
-        const int row = int(uint32_t(at) / uint32_t(p.divisor));
-        return at >= 0 && row < p.x_rows ? row : -1;
+    // The tile's row ml in x, or -1 (past the group, or an order entry outside x), in
+    // two parts: the load, which other loads need not wait for (without an order
+    // it reads an offset), and the row.
+    const int *entries = p.order ? p.order + m_base : p.offsets;
+    auto entry = [&](int ml) { return entries[p.order ? min(ml, tile.rows - 1) : 0]; };
+    auto source = [&](int at, int ml) {
+        const int row = p.order ? int(uint32_t(at) / uint32_t(p.divisor)) : m_base + ml;
+        return ml < tile.rows && (!p.order || at >= 0) && row < p.x_rows ? row : -1;
     };
 
     const int k_begin = ks * steps * BK;
@@ -99,9 +100,13 @@ __global__ __launch_bounds__(64 * KS * WN * WM, EU) void expert_gemm(ExpertArgs 
     const uint32_t woff0 = uint32_t(lane_row) * uint32_t(K) + uint32_t(chunk0 * 16);
     const uint32_t woff1 = uint32_t(lane_row) * uint32_t(K) + uint32_t(chunk1 * 16);
     constexpr uint32_t kOut = 0x80000000u;  // an offset past every buffer: reads as zero
-    int xrow[XI];
+    auto x_ml = [&](int i) { return (NWS > 1 ? i * NWS + ws : i) * 8 + lane_row; };
+    auto s_ml = [&](int i) { return (i * NWS + ws - 1) * 64 + lane; };
+    int x_entry[XI], s_entry[SI + 1], to_entry = entry(tid);
 #pragma unroll
-    for (int i = 0; i < XI; ++i) xrow[i] = source((NWS > 1 ? i * NWS + ws : i) * 8 + lane_row);
+    for (int i = 0; i < XI; ++i) x_entry[i] = entry(x_ml(i));
+#pragma unroll
+    for (int i = 0; i < SI; ++i) s_entry[i] = entry(max(s_ml(i), 0));
     uint8_t *ring = lds + ks * S * STAGE;
     uint8_t *dma_base = ring;
     uint32_t dk = 0;
@@ -109,7 +114,7 @@ __global__ __launch_bounds__(64 * KS * WN * WM, EU) void expert_gemm(ExpertArgs 
     auto aim = [&](int st, int slot) {
         dma_base = ring + slot * STAGE;
         dk = uint32_t(k_begin + st * BK);
-        in0 = int(dk) + chunk0 * 16 < K, in1 = int(dk) + chunk1 * 16 < K;
+        in0 = st < count && int(dk) + chunk0 * 16 < K, in1 = st < count && int(dk) + chunk1 * 16 < K;
     };
     auto dma_w = [&](auto j_) {
         constexpr int j = decltype(j_)::value;
@@ -127,26 +132,22 @@ __global__ __launch_bounds__(64 * KS * WN * WM, EU) void expert_gemm(ExpertArgs 
         __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc_x, (lds_ptr_t)(dma_base + (BN / 8 + g) * 1024), 16, at,
                                                  dk, 0, 0);
     };
-    // Where all of a slice's stages fit its ring, their weights are asked for
-    // before the rows' addresses are known (those wait for the offsets, then
-    // the order).
-    const bool whole = count <= S;
-    __builtin_amdgcn_sched_barrier(0);
-    if (whole) {
+    // The first S stages: their weights are asked for before the rows' addresses
+    // are known (those wait for the offsets, then the order). Stages that the slice
+    // does not have are asked for as zeros, so that every wave's count of loads in
+    // flight is known and no wait is longer than it has to be.
+    pin();
 #pragma unroll
-        for (int s = 0; s < S; ++s)
-            if (s < count) {
-                aim(s, s);
-                static_for<0, WI>(dma_w);
-            }
-        __builtin_amdgcn_sched_barrier(0);
+    for (int s = 0; s < S; ++s) {
+        aim(s, s);
+        static_for<0, WI>(dma_w);
     }
+    pin();
 #pragma unroll
     for (int i = 0; i < XI; ++i) {
-        const int chunk = NWS > 1 || !(i & 1) ? chunk0 : chunk1;
-        xoff[i] = xrow[i] < 0 ? kOut
-                              : uint32_t(p.order ? xrow[i] : xrow[i] - m_base) * uint32_t(K) +
-                                    uint32_t(chunk * 16);
+        const int chunk = NWS > 1 || !(i & 1) ? chunk0 : chunk1, row = source(x_entry[i], x_ml(i));
+        xoff[i] = row < 0 ? kOut
+                          : uint32_t(p.order ? row : row - m_base) * uint32_t(K) + uint32_t(chunk * 16);
     }
 
     // K groups: a stage's scales arrive with it, [BN] then [BM] floats behind its
@@ -159,8 +160,8 @@ __global__ __launch_bounds__(64 * KS * WN * WM, EU) void expert_gemm(ExpertArgs 
     uint32_t soff[SI + 1];
 #pragma unroll
     for (int i = 0; i < SI; ++i) {
-        const int q = i * NWS + ws, ml = (q - 1) * 64 + lane;
-        const int row = q > 0 && ml < BM ? source(ml) : -1;
+        const int q = i * NWS + ws, ml = s_ml(i);
+        const int row = q > 0 && ml < BM ? source(s_entry[i], ml) : -1;
         soff[i] = q == 0 ? (lane * 4 < BN && n_base + lane * 4 < N ? uint32_t(lane * 16) : kOut)
                   : row < 0 ? kOut : uint32_t(row) * 4u;
     }
@@ -184,22 +185,15 @@ __global__ __launch_bounds__(64 * KS * WN * WM, EU) void expert_gemm(ExpertArgs 
         else dma_s(std::integral_constant<int, i < WI + XI ? 0 : i - WI - XI>{});
     };
 
-    // For the epilogue, in LDS past the ring: the rows' scales and where they go, the
-    // channels' scales.
+    // For the epilogue: a row's scale and where it goes, a channel's scale, one each
+    // per thread until the walk is done (a wait for them here would wait for the
+    // weights), then in LDS past the ring.
+    static_assert(BM <= 64 * W && BN <= 64 * W, "one row and one channel per thread");
     constexpr int kBody = expert_body_bytes(Grouped, KS, S, BN, BM);
     float *row_scale = reinterpret_cast<float *>(lds + kBody), *col_scale = row_scale + BM;
     int *row_to = reinterpret_cast<int *>(col_scale + BN);
-    for (int i = tid; i < BM; i += 64 * W) {
-        const int from = source(i);
-        int to = i < tile.rows ? m_base + i : -1;
-        if (p.scatter && to >= 0) {
-            to = p.order[to];
-            if (uint32_t(to) >= uint32_t(p.slots)) to = -1;
-        }
-        row_to[i] = to;
-        row_scale[i] = Grouped ? 1.f : p.sx[max(from, 0)];
-    }
-    for (int i = tid; i < BN; i += 64 * W) col_scale[i] = Grouped ? 1.f : sw[min(n_base + i, N - 1)];
+    const float row_scale_v = Grouped ? 1.f : p.sx[max(source(to_entry, tid), 0)];
+    const float col_scale_v = Grouped ? 1.f : sw[min(n_base + tid, N - 1)];
 
     using Sum = std::conditional_t<Grouped, f32x4, Acc>;
     Sum acc[NF][MT];
@@ -253,31 +247,15 @@ __global__ __launch_bounds__(64 * KS * WN * WM, EU) void expert_gemm(ExpertArgs 
         }
     };
 
-    // The rest of the first stages' DMA.
+    // The rest of the first stages' loads.
     pin();
 #pragma unroll
-    for (int s = 0; s < S; ++s)
-        if (s < count) {
-            aim(s, s);
-            if (!whole) static_for<0, WI>(dma_w);
-            static_for<0, XI>(dma_x);
-            static_for<0, SI>(dma_s);
-        }
-    // Wait for stage `st` with `newer` later ones asked for.
-    auto wait_stage = [&](int newer) {
-        if (whole) {
-            if (newer >= 3 && S > 3) wait_vmcnt<(XI + SI) * 3>();
-            else if (newer == 2) wait_vmcnt<(XI + SI) * 2>();
-            else if (newer == 1) wait_vmcnt<XI + SI>();
-            else wait_vmcnt<0>();
-        } else {
-            if (newer >= 3 && S > 3) wait_vmcnt<INSTS * 3>();
-            else if (newer == 2) wait_vmcnt<INSTS * 2>();
-            else if (newer == 1) wait_vmcnt<INSTS>();
-            else wait_vmcnt<0>();
-        }
-    };
-    static_assert(S <= 4, "the waits above");
+    for (int s = 0; s < S; ++s) {
+        aim(s, s);
+        static_for<0, XI>(dma_x);
+        static_for<0, SI>(dma_s);
+    }
+    static_assert(S == 2 || S == 3, "the waits below");
     int slot = 0;  // of the stage whose token fragments are in registers
     // Step s: at its start every read of stage s - 1 has arrived (with a shared
     // ring in every wave), so that stage's slot takes stage s - 1 + S. Weight
@@ -297,7 +275,11 @@ __global__ __launch_bounds__(64 * KS * WN * WM, EU) void expert_gemm(ExpertArgs 
             pin();  // (a stage's weight fragments at once do not fit the registers)
         });
         slot = slot + 1 == S ? 0 : slot + 1;
-        if (s + 1 < count) wait_stage(min(s - 1 + S, count - 1) - (s + 1));
+        if (s + 1 < count) {  // stage s + 1, with at most one later one in flight
+            if (s == 0) wait_vmcnt<(XI + SI) * (S - 2)>();
+            else if (S == 3 && s + 2 < count) wait_vmcnt<INSTS>();
+            else wait_vmcnt<0>();
+        }
         pin();
         wait_lds_reads();
         if constexpr (NWS > 1) __builtin_amdgcn_s_barrier();
@@ -317,7 +299,7 @@ __global__ __launch_bounds__(64 * KS * WN * WM, EU) void expert_gemm(ExpertArgs 
         i32x8 a, b0[L], b1[L];
         f32x4 aw;
         float x0[L], x1[L];
-        wait_stage(min(S, count) - 1);
+        wait_vmcnt<(XI + SI) * (S - 1)>();
         if constexpr (NWS > 1) __builtin_amdgcn_s_barrier();
         pin();
         read_x(0, b0);
@@ -350,6 +332,13 @@ __global__ __launch_bounds__(64 * KS * WN * WM, EU) void expert_gemm(ExpertArgs 
         }
     }
     static_assert(MT == 1 || MT == 2 || MT == 4, "the walks above");
+    if (tid < BM) {
+        const int to = p.scatter ? to_entry : m_base + tid;
+        row_to[tid] = tid < tile.rows && uint32_t(to) < uint32_t(p.slots) ? to : -1;
+        row_scale[tid] = row_scale_v;
+    }
+    if (tid < BN) col_scale[tid] = col_scale_v;
+    wait_vmcnt<0>();  // (stages past the walk's end still write zeros)
     wait_lds_reads();
     __syncthreads();
 

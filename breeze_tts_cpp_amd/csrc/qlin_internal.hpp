@@ -226,7 +226,9 @@ struct AdapterArgs {
     const void *base;    // [rows, ldy] or null
     void *y;             // [rows, ldy]
     int ldx, ldy, rows, adapters, rank, N, K, type;
+    void *workspace;     // adapter_workspace_bytes
 };
+size_t adapter_workspace_bytes(int rows, int adapters, int K, int rank);
 void launch_adapter(const AdapterArgs &, hipStream_t);
 
 // Records `message` as qlin_last_error() of this thread; returns status.

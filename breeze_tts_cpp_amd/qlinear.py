@@ -76,7 +76,8 @@ EXPORTS = ("qlin_version", "qlin_last_error", "qlin_row_quantize", "qlin_plan",
            "qlin_norm_fusion_init", "qlin_epilogue_init", "qlin_layer_norm_quantize",
            "qlin_pointwise_quantize", "qlin_pointwise", "qlin_linear_noalloc", "qlin_noalloc_scratch_bytes",
            "qlin_group_rows_workspace_bytes", "qlin_group_rows", "qlin_route", "qlin_combine",
-           "qlin_expert_plan", "qlin_expert_gemm", "qlin_adapter_add")
+           "qlin_expert_plan", "qlin_expert_gemm", "qlin_adapter_workspace_bytes",
+           "qlin_adapter_add")
 
 
 def load():
@@ -150,8 +151,10 @@ def load():
     L.qlin_expert_gemm.restype = i
     L.qlin_expert_gemm.argtypes = [ctypes.POINTER(qlin_path), P, P, i, P, i, P, P, P, i, P, i, i, i,
                                    i, i, i, i, P]
+    L.qlin_adapter_workspace_bytes.restype = sz
+    L.qlin_adapter_workspace_bytes.argtypes = [i, i, i, i]
     L.qlin_adapter_add.restype = i
-    L.qlin_adapter_add.argtypes = [P, i, P, P, i, i, P, P, i, P, P, P, P, i, i, i, i, P]
+    L.qlin_adapter_add.argtypes = [P, i, P, P, i, i, P, P, i, P, P, P, P, i, i, i, i, P, sz, P]
     _lib = L
     return L
 
@@ -716,9 +719,14 @@ def expert_gemm(xq: torch.Tensor, sx: torch.Tensor, wq: torch.Tensor, sw: torch.
     return out
 
 
+def adapter_workspace_bytes(rows: int, adapters: int, K: int, rank: int) -> int:
+    return int(load().qlin_adapter_workspace_bytes(rows, adapters, K, rank))
+
+
 def adapter_add(x: torch.Tensor, order: torch.Tensor, offsets: torch.Tensor, a: torch.Tensor,
                 b: torch.Tensor, y: torch.Tensor, base: torch.Tensor | None = None,
-                ranks: torch.Tensor | None = None, scales: torch.Tensor | None = None, stream=None):
+                ranks: torch.Tensor | None = None, scales: torch.Tensor | None = None,
+                workspace: torch.Tensor | None = None, stream=None):
     """Low-rank adapters beside a shared projection (qlin_adapter_add): rows of
     adapter g get y = base + scales[g] * (x a[g]^T) b[g]^T in x's 16-bit type;
     a [adapters, rank, K], b [adapters, N, rank], order / offsets of
@@ -748,8 +756,11 @@ def adapter_add(x: torch.Tensor, order: torch.Tensor, offsets: torch.Tensor, a: 
         _indices(ranks, "ranks", adapters)
     if scales is not None:
         _floats(scales, "scales", adapters)
-    _on_device(x, order, offsets, a, b, y, base, ranks, scales)
+    need = 0 if workspace is not None else L.qlin_adapter_workspace_bytes(rows, adapters, K, rank)
+    workspace, ws_ptr, ws_bytes = _buffer(workspace, need, x.device, stream)
+    _on_device(x, order, offsets, a, b, y, base, ranks, scales, workspace)
     _check(L.qlin_adapter_add(x.data_ptr(), ldx, order.data_ptr(), offsets.data_ptr(), rows, adapters,
                               a.data_ptr(), b.data_ptr(), rank, _ptr(ranks), _ptr(scales),
-                              base.data_ptr(), y.data_ptr(), ldy, N, K, kind, _stream(stream)))
+                              base.data_ptr(), y.data_ptr(), ldy, N, K, kind, ws_ptr, ws_bytes,
+                              _stream(stream)))
     return y

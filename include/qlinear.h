@@ -33,7 +33,7 @@
  *                          scratch in a fixed library-owned device array, for callers
  *                          that cannot allocate
  *   qlin_route, qlin_group_rows, qlin_combine, qlin_expert_gemm, qlin_expert_plan,
- *   qlin_adapter_add, qlin_group_rows_workspace_bytes
+ *   qlin_adapter_add and their workspace sizes
  *                       <- no counterpart in the reference: rows that each name the
  *                          weights they use (experts, codebook heads, adapters)
  *
@@ -431,10 +431,11 @@ int qlin_expert_gemm(const qlin_path *path, const void *x, const float *sx, int 
  * row at most once.
  * A column range of y (one projection of a merged output) is a y offset by its
  * first column with the whole row's ldy. */
+size_t qlin_adapter_workspace_bytes(int rows, int adapters, int K, int rank);
 int qlin_adapter_add(const void *x, int ldx, const int *order, const int *offsets, int rows,
                      int adapters, const void *a, const void *b, int rank, const int *ranks,
                      const float *scales, const void *base, void *y, int ldy, int N, int K, int type,
-                     qlin_stream_t stream);
+                     void *workspace, size_t workspace_bytes, qlin_stream_t stream);
 
 #ifdef __cplusplus
 }

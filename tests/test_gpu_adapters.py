@@ -162,3 +162,15 @@ def test_row_does_not_depend_on_its_place(dev):
             order, _, offsets = qlinear.group_rows(ids[p].to(dev), 4)
             outs.append(qlinear.adapter_add(x[p].to(dev), order, offsets, a, b, y[p].to(dev)).cpu())
         assert torch.equal(outs[0][perm], outs[1])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("rows,adapters,rank,N,K", [(2300, 3, 40, 272, 6160), (4096, 6, 64, 528, 4096),
+                                                    (1500, 40, 128, 144, 4112), (6000, 2, 16, 96, 6144)])
+def test_two_launches(dev, dtype, rows, adapters, rank, N, K):
+    """Sizes of the form with a workspace, ranks off the 8, one adapter short of rows."""
+    from breeze_tts_cpp_amd import qlinear
+    assert qlinear.adapter_workspace_bytes(rows, adapters, K, rank) > 0
+    run_case(dev, rows, adapters, rank, N, K, dtype, runs=rows // (adapters * 2) + 1)
+    run_case(dev, rows, adapters, rank, N, K, dtype, runs=7, xpad=3, ypad=1, base="separate",
+             ranks=[rank, 0, rank // 2 + 1] + [3] * (adapters - 3) if adapters > 2 else [rank, 5])

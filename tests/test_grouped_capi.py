@@ -106,9 +106,9 @@ def test_adapter_refusals():
     L = qlinear.load()
 
     def call(x=FAKE, ldx=256, order=FAKE, off=FAKE, rows=8, n=4, a=FAKE, b=FAKE, rank=16, ranks=None,
-             scales=None, base=None, y=FAR, ldy=64, N=64, K=256, t=BF16):
+             scales=None, base=None, y=FAR, ldy=64, N=64, K=256, t=BF16, ws=None, wsb=0):
         return L.qlin_adapter_add(x, ldx, order, off, rows, n, a, b, rank, ranks, scales, base, y,
-                                  ldy, N, K, t, None)
+                                  ldy, N, K, t, ws, wsb, None)
 
     assert call(t=F32) == -1 and call(rows=0) == -1 and call(N=40) == -1 and call(K=200) == -1
     assert call(ldx=255) == -1 and call(ldy=63) == -1
@@ -120,8 +120,13 @@ def test_adapter_refusals():
     assert call(order=FAKE + 2) == -2 and call(scales=FAKE + 1) == -2 and call(ranks=FAKE + 2) == -2
     assert call(y=FAKE + 64) == -1 and b"overlaps" in L.qlin_last_error()
     assert call(base=FAR + 2) == -1
-    assert call(rows=1 << 22) == -4 and b"2 GiB" in L.qlin_last_error()
-    assert call(rows=1 << 25, N=1 << 20, ldy=1 << 20, K=16, ldx=16, x=1 << 60) == -4
+    need = L.qlin_adapter_workspace_bytes(4096, 4, 6144, 64)
+    assert need > 0 and L.qlin_adapter_workspace_bytes(1, 4, 6144, 64) == 0
+    big = dict(rows=4096, K=6144, ldx=6144, rank=64)
+    assert call(**big) == -3 and call(ws=FAKE, wsb=need - 1, **big) == -3
+    assert call(ws=FAKE + 4, wsb=need, **big) == -2
+    assert call(rows=1 << 22, ws=FAKE, wsb=1 << 60) == -4 and b"2 GiB" in L.qlin_last_error()
+    assert call(rows=1 << 25, N=1 << 20, ldy=1 << 20, K=16, ldx=16, x=1 << 60, ws=FAKE, wsb=1 << 60) == -4
     assert b"tiles" in L.qlin_last_error()
 
 
