@@ -62,46 +62,43 @@ int check_grouping(const char *what, const int *ids, long count, int groups, con
 // of whose sizes the host knows no more than their mean. Measured with uneven
 // groups (weights from HBM, 80 shapes of 8-64 experts, 1024-4096 channels, K
 // 1024-4096, 0.25-1024 rows per expert, INT8 and group FP8):
-//  - up to 8 rows per expert the weights' bytes are all: 64x32 tiles, two or three
-//    workgroups per CU (32 experts of 2048 x 2048, 4 rows each: 25 us, 28 with the
+//  - up to 8 rows per expert the weights' bytes are all: 64x32 tiles, two
+//    workgroups per CU (32 experts of 2048 x 2048, 4 rows each: 24.6 us, 26.7 with the
 //    K-sliced 32x16 tile). Where they would leave CUs without work, the K-sliced
 //    tile has twice the workgroups, each a quarter of the K walk (16 of 1024 x
-//    4096, 1 row: 11.2 us against 16.3; 8 of 64, 2048 x 2048: 8.5 against 9.3; with K
+//    4096, 1 row: 10.2 us against 13.0; 8 of 64, 2048 x 2048: 8.4 against 8.9; with K
 //    groups only from K above 2048: 11.9 against 10.3 at 2048);
-//  - up to 96 rows 128x64 (16 rows: 27.8 us against 31.7 on 64x32, 31.5 on 128x128),
+//  - up to 96 rows 128x64 (16 rows: 27.7 us against 30.0 on 64x32, 31.3 on 256x128),
 //    but 64x32 up to 32 rows where 128-channel tiles leave CUs without work (16 of
-//    1024 x 4096, 16 rows: 21.2 against 24.1);
+//    1024 x 4096, 16 rows: 20.8 against 23.8);
 //  - above, the tile whose rounds of workgroups cost least, at the time that a
 //    round of each takes with uneven groups (128x64: two workgroups per CU), a part
-//    per 128 of K and a fixed one (prologue, epilogue).
-// With K groups 128x64 from 4 rows (6 rows, 31 experts of 2064 x 2048: 23.3 us, 26.3 on
-// 64x32). On the 80 shapes the choice is within 6% of the best tile.
+//    per 128 of K and a fixed one (prologue, epilogue). A 128x128 tile, two
+//    workgroups per CU, was best by at most 5%, for 128-256 rows of short K.
+// With K groups 128x64 from 4 rows (6 rows, 31 experts of 2064 x 2048: 23.5 us, 26.7 on
+// 64x32), at any size (a 128x128 tile gains 15% at most, one round of long K).
+// On the 80 shapes the choice is within 7% of the best tile but for three (9-15%).
 int choose_tile(long slots, int experts, int N, int K, int group) {
     const long each = slots / experts;
     const long some = slots < experts ? slots : experts;  // groups that can have rows
     if (each <= 8 && some * ((N + 63) / 64) <= 256 && (!group || K > 2048)) return 0;
     if (each <= (group ? 3 : 8)) return 1;
     if (each <= 32 && some * ((N + 127) / 128) < 256) return 1;
-    if (each <= 96) return 2;
-    constexpr struct { int tile, per_round, stage, fixed, grouped_stage, grouped_fixed; } kCost[] = {
-        {2, 512, 740, 4000, 1020, 2600},
-        {3, 256, 650, 4300, 825, 4500},
-        {4, 256, 975, 7500, 0, 0},
-        {5, 256, 1810, 9900, 0, 0}};  // ns
+    if (each <= 96 || group) return 2;
+    constexpr struct { int tile, per_round, stage, fixed; } kCost[] = {
+        {2, 512, 755, 3200}, {3, 256, 950, 7200}, {4, 256, 1765, 9500}};  // ns
     const long stages = (long(K) + 127) / 128;
     int best = 2;
     long least = LONG_MAX;
     for (const auto &c : kCost) {
         const auto &t = qlin::kExpertTiles[c.tile];
-        if (group && !c.grouped_stage) continue;
         // A group's last tile is short: on average 0.6 of a tile more, at least one.
         const long rows = slots / t.tokens + experts * 3L / 5;
         const long tiles = (rows > experts ? rows : experts) * ((N + t.channels - 1) / t.channels);
         // Whole rounds while they are few; many even out to half a round more.
         const long rounds2 = tiles <= 4 * c.per_round ? (tiles + c.per_round - 1) / c.per_round * 2
                                                       : tiles * 2 / c.per_round + 1;
-        const long cost = rounds2 * (group ? stages * c.grouped_stage + c.grouped_fixed
-                                           : stages * c.stage + c.fixed);
+        const long cost = rounds2 * (stages * c.stage + c.fixed);
         if (cost < least) least = cost, best = c.tile;
     }
     return best;

@@ -194,12 +194,11 @@ struct ExpertArgs {
 #define QLIN_EXPERT_TILES(X)  \
     X(0, 4, 1, 1, 2, 1, 3, 2) \
     X(1, 1, 4, 1, 1, 2, 3, 4) \
-    X(2, 1, 4, 2, 2, 2, 3, 4) \
-    X(3, 1, 2, 4, 4, 2, 3, 2)
+    X(2, 1, 4, 2, 2, 2, 3, 4)
 #define QLIN_EXPERT_WIDE_TILES(X) \
-    X(4, 1, 4, 2, 4, 4, 3, 2)     \
-    X(5, 1, 2, 4, 8, 4, 2, 2)
-constexpr int kExpertNarrowTiles = 4;
+    X(3, 1, 4, 2, 4, 4, 3, 2)     \
+    X(4, 1, 2, 4, 8, 4, 2, 2)
+constexpr int kExpertNarrowTiles = 3;
 struct ExpertTile {
     int channels, tokens, waves, slices;
 };

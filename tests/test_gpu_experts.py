@@ -78,7 +78,7 @@ def every_path():
                         p = qlinear.expert_plan(slots, experts, N, K, fmt, group)
                         if (mode, p) not in seen:
                             seen.append((mode, p))
-    assert len(seen) == 20  # six tiles per channel, four with K groups
+    assert len(seen) == 16  # five tiles per channel, three with K groups
     return seen
 
 
