@@ -447,7 +447,7 @@ int set_error(int status, const char *message) { return fail(status, "%s", messa
 
 extern "C" {
 
-int qlin_version(void) { return 101; }
+int qlin_version(void) { return 102; }
 
 const char *qlin_last_error(void) { return g_error; }
 

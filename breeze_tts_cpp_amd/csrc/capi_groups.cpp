@@ -36,6 +36,16 @@ bool overlap(const void *a, size_t an, const void *b, size_t bn) {
     return x < y + bn && y < x + an;
 }
 
+// So do rows of `an` and `bn` columns, strides lda and ldb (16-bit elements). Column
+// ranges of the same wider rows do not.
+bool rows_overlap(const void *a, int lda, int an, const void *b, int ldb, int bn, int rows) {
+    if (!overlap(a, (size_t(rows - 1) * lda + an) * 2, b, (size_t(rows - 1) * ldb + bn) * 2)) return false;
+    if (rows == 1 || lda != ldb) return true;
+    const intptr_t apart = (reinterpret_cast<intptr_t>(b) - reinterpret_cast<intptr_t>(a)) / 2;
+    const intptr_t column = (apart % lda + lda) % lda;  // of b's first element in a's rows
+    return column < an || column + bn > lda;
+}
+
 // Most ids of one grouping (index arithmetic past the last run stays in int).
 constexpr int kMaxIds = 1 << 30;
 
@@ -49,6 +59,13 @@ int check_grouping(const char *what, const int *ids, long count, int groups, con
         return fail(QLIN_ERR_INVALID, "%s: null pointer", what);
     if (!aligned(ids, 4) || !aligned(order, 4) || !aligned(slots, 4) || !aligned(offsets, 4))
         return fail(QLIN_ERR_ALIGNMENT, "%s: index arrays must be 4-byte aligned", what);
+    const size_t flat = size_t(count) * 4;
+    const struct { const void *p; size_t bytes; } arrays[] = {
+        {ids, flat}, {order, flat}, {slots, flat}, {offsets, size_t(groups + 1) * 4}};
+    for (int i = 0; i < 4; ++i)
+        for (int j = 0; j < i; ++j)
+            if (overlap(arrays[i].p, arrays[i].bytes, arrays[j].p, arrays[j].bytes))
+                return fail(QLIN_ERR_INVALID, "%s: ids, order, slots and offsets overlap", what);
     const size_t need = qlin::group_workspace_bytes(int(count), groups);
     if (need && (!workspace || bytes < need))
         return fail(QLIN_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", what, need,
@@ -85,11 +102,11 @@ int choose_tile(long slots, int experts, int N, int K, int group) {
     if (each <= (group ? 3 : 8)) return 1;
     if (each <= 32 && some * ((N + 127) / 128) < 256) return 1;
     if (each <= 96 || group) return 2;
-    constexpr struct { int tile, per_round, stage, fixed; } kCost[] = {
+    constexpr struct { int tile; long per_round; double stage, fixed; } kCost[] = {
         {2, 512, 755, 3200}, {3, 256, 950, 7200}, {4, 256, 1765, 9500}};  // ns
-    const long stages = (long(K) + 127) / 128;
+    const double stages = double((long(K) + 127) / 128);
     int best = 2;
-    long least = LONG_MAX;
+    double least = 1e300;
     for (const auto &c : kCost) {
         const auto &t = qlin::kExpertTiles[c.tile];
         // A group's last tile is short: on average 0.6 of a tile more, at least one.
@@ -98,7 +115,7 @@ int choose_tile(long slots, int experts, int N, int K, int group) {
         // Whole rounds while they are few; many even out to half a round more.
         const long rounds2 = tiles <= 4 * c.per_round ? (tiles + c.per_round - 1) / c.per_round * 2
                                                       : tiles * 2 / c.per_round + 1;
-        const long cost = rounds2 * (stages * c.stage + c.fixed);
+        const double cost = double(rounds2) * (stages * c.stage + c.fixed);
         if (cost < least) least = cost, best = c.tile;
     }
     return best;
@@ -166,6 +183,15 @@ int qlin_route(const void *logits, int ld, int logits_type, int tokens, int expe
     const int status = check_grouping("router", ids, long(tokens) * top_k, experts, order, slots,
                                       offsets, workspace, workspace_bytes);
     if (status) return status;
+    const size_t logits_bytes = (size_t(tokens - 1) * ld + experts) * (logits_type == QLIN_F32 ? 4 : 2);
+    const size_t flat = size_t(tokens) * top_k * 4, index_bytes[] = {flat, flat, flat, size_t(experts + 1) * 4};
+    const void *index[] = {ids, order, slots, offsets};
+    for (int i = 0; i < 4; ++i)
+        if (overlap(index[i], index_bytes[i], logits, logits_bytes) ||
+            overlap(index[i], index_bytes[i], weights, flat))
+            return fail(QLIN_ERR_INVALID, "router outputs overlap its logits or each other");
+    if (overlap(weights, flat, logits, logits_bytes))
+        return fail(QLIN_ERR_INVALID, "router outputs overlap its logits or each other");
     qlin::launch_route({logits, ld, logits_type, tokens, experts, top_k, normalize != 0, ids, weights},
                        {ids, tokens * top_k, experts, order, slots, offsets, workspace},
                        reinterpret_cast<hipStream_t>(stream));
@@ -225,6 +251,8 @@ int qlin_expert_gemm(const qlin_path *path, const void *x, const float *sx, int 
         return fail(QLIN_ERR_ALIGNMENT, "scales must be 4-byte aligned (group weight scales 16-byte)");
     if (!aligned(offsets, 4) || !aligned(order, 4))
         return fail(QLIN_ERR_ALIGNMENT, "index arrays must be 4-byte aligned");
+    if (overlap(x, size_t(x_rows) * K, y, size_t(slots) * N * 2))
+        return fail(QLIN_ERR_INVALID, "grouped GEMM output overlaps its input");
     // Gathered rows are addressed through one 32-bit buffer range, and so are a
     // tile's rows of either operand.
     if (order && long(x_rows) * K > INT32_MAX)
@@ -282,10 +310,10 @@ int qlin_adapter_add(const void *x, int ldx, const int *order, const int *offset
         return fail(QLIN_ERR_ALIGNMENT, "16-bit rows must be 2-byte aligned");
     if (!aligned(order, 4) || !aligned(offsets, 4) || !aligned(ranks, 4) || !aligned(scales, 4))
         return fail(QLIN_ERR_ALIGNMENT, "index arrays and scales must be 4-byte aligned");
-    const size_t x_bytes = (size_t(rows - 1) * ldx + K) * 2, y_bytes = (size_t(rows - 1) * ldy + N) * 2;
-    if (overlap(x, x_bytes, y, y_bytes))
+    const size_t x_bytes = (size_t(rows - 1) * ldx + K) * 2;
+    if (rows_overlap(x, ldx, K, y, ldy, N, rows))
         return fail(QLIN_ERR_INVALID, "adapter output overlaps its input");
-    if (base && base != y && overlap(base, y_bytes, y, y_bytes))
+    if (base && base != y && rows_overlap(base, ldy, N, y, ldy, N, rows))
         return fail(QLIN_ERR_INVALID, "adapter output overlaps part of its base");
     const size_t need = qlin::adapter_workspace_bytes(rows, adapters, K, rank);
     if (need && (!workspace || workspace_bytes < need))

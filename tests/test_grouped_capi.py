@@ -10,12 +10,14 @@ from breeze_tts_cpp_amd import qlinear
 BF16, F32, I32, FP8, I8, F16 = 0, 1, 2, 3, 4, 5
 FAKE = 0x10000  # never dereferenced
 FAR = 0x40000000000
+# Addresses far apart, for arrays that must not overlap.
+IDS, ORDER, SLOTS, OFFSETS, WEIGHTS = (FAR * k for k in range(2, 7))
 
 
 def test_group_rows_refusals():
     L = qlinear.load()
 
-    def call(ids=FAKE, count=100, groups=8, order=FAKE, slots=FAKE, offsets=FAKE, ws=None, wsb=0):
+    def call(ids=IDS, count=100, groups=8, order=ORDER, slots=SLOTS, offsets=OFFSETS, ws=None, wsb=0):
         return L.qlin_group_rows(ids, count, groups, order, slots, offsets, ws, wsb, None)
 
     assert call(count=0) == -1 and call(count=(1 << 30) + 1) == -1
@@ -23,6 +25,8 @@ def test_group_rows_refusals():
     for name in ("ids", "order", "slots", "offsets"):
         assert call(**{name: None}) == -1
         assert call(**{name: FAKE + 2}) == -2
+    assert call(slots=IDS) == -1 and b"overlap" in L.qlin_last_error()
+    assert call(order=IDS + 396) == -1 and call(offsets=SLOTS - 32) == -1
     need = L.qlin_group_rows_workspace_bytes(100000, 8)
     assert need > 0 and L.qlin_group_rows_workspace_bytes(4096, 1024) == 0
     assert call(count=100000) == -3 and b"workspace" in L.qlin_last_error()
@@ -35,8 +39,8 @@ def test_group_rows_refusals():
 def test_route_refusals():
     L = qlinear.load()
 
-    def call(logits=FAKE, ld=64, t=F32, tokens=4, experts=64, k=2, ids=FAKE, w=FAKE, order=FAKE,
-             slots=FAKE, off=FAKE, ws=None, wsb=0):
+    def call(logits=FAKE, ld=64, t=F32, tokens=4, experts=64, k=2, ids=IDS, w=WEIGHTS, order=ORDER,
+             slots=SLOTS, off=OFFSETS, ws=None, wsb=0):
         return L.qlin_route(logits, ld, t, tokens, experts, k, 0, ids, w, order, slots, off, ws, wsb,
                             None)
 
@@ -45,7 +49,8 @@ def test_route_refusals():
     assert call(k=0) == -1 and call(k=17) == -1 and call(experts=3, k=4) == -1
     for name in ("logits", "ids", "w", "order", "slots", "off"):
         assert call(**{name: None}) == -1
-    assert call(logits=FAKE + 2) == -2 and call(w=FAKE + 2) == -2
+    assert call(logits=FAKE + 2) == -2 and call(w=WEIGHTS + 2) == -2
+    assert call(w=FAKE + 4) == -1 and call(ids=FAKE + 1020) == -1 and call(w=SLOTS) == -1
     assert call(t=BF16, logits=FAKE + 1) == -2
     assert call(tokens=4096, k=2) == -3
     assert call(tokens=1 << 29, k=8) == -1  # more choices than an index holds
@@ -71,7 +76,7 @@ def test_expert_refusals():
     L = qlinear.load()
 
     def call(path=None, x=FAKE, sx=FAKE, x_rows=64, order=FAKE, div=1, off=FAKE, w=FAKE, sw=FAKE,
-             experts=8, y=FAKE, scatter=0, slots=64, N=64, K=256, fmt=I8, out=BF16, group=0):
+             experts=8, y=FAR, scatter=0, slots=64, N=64, K=256, fmt=I8, out=BF16, group=0):
         p = ctypes.byref(path.to_c()) if path else None
         return L.qlin_expert_gemm(p, x, sx, x_rows, order, div, off, w, sw, experts, y, scatter,
                                   slots, N, K, fmt, out, group, None)
@@ -85,7 +90,8 @@ def test_expert_refusals():
     assert call(div=0) == -1
     assert call(order=None, scatter=1) == -1
     assert call(order=None, x_rows=63) == -1 and call(x_rows=0) == -1
-    assert call(x=FAKE + 8) == -2 and call(w=FAKE + 8) == -2 and call(y=FAKE + 4) == -2
+    assert call(x=FAKE + 8) == -2 and call(w=FAKE + 8) == -2 and call(y=FAR + 4) == -2
+    assert call(y=FAKE + 64 * 256 - 16) == -1 and b"overlaps" in L.qlin_last_error()
     assert call(sx=FAKE + 2) == -2 and call(sw=FAKE + 4, group=128) == -2
     assert call(order=FAKE + 2) == -2
     assert call(x_rows=1 << 20, K=2048) == -4 and b"2 GiB" in L.qlin_last_error()
@@ -120,6 +126,12 @@ def test_adapter_refusals():
     assert call(order=FAKE + 2) == -2 and call(scales=FAKE + 1) == -2 and call(ranks=FAKE + 2) == -2
     assert call(y=FAKE + 64) == -1 and b"overlaps" in L.qlin_last_error()
     assert call(base=FAR + 2) == -1
+    # Column ranges of the same wider rows are apart, or they overlap (rows too many
+    # for the call stand for "passed this check").
+    wide = dict(ldx=512, ldy=512, rows=1 << 22, ws=FAKE, wsb=1 << 60)
+    for apart, status in ((256, -4), (448, -4), (255, -1), (449, -1), (-64, -4), (-63, -1), (0, -1)):
+        assert call(y=FAKE + 2 * apart, **wide) == status, apart
+    assert call(y=FAKE + 512, **dict(wide, ldy=520)) == -1  # not the same rows
     need = L.qlin_adapter_workspace_bytes(4096, 4, 6144, 64)
     assert need > 0 and L.qlin_adapter_workspace_bytes(1, 4, 6144, 64) == 0
     big = dict(rows=4096, K=6144, ldx=6144, rank=64)
