@@ -547,23 +547,15 @@ def linear_noalloc(x: torch.Tensor, wq: torch.Tensor, sw: torch.Tensor, fmt: int
 
 # ---------------------------------------------------------------- rows grouped by weights
 # These run between the products of a decode step, where a call's time on the
-# host is what counts (a launch alone is about 4 us of it): checks read plain
-# tensor attributes, and buffers are made in their final shape.
+# host is what counts (of 7 us the launch is 3): checks read plain tensor
+# attributes, in line, and buffers are made in their final shape.
 _LOGITS = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
-_int32 = torch.int32
-_current_device = torch.cuda.current_device
+_int32, _f32 = torch.int32, torch.float32
+_empty, _current_device = torch.empty, torch.cuda.current_device
 
 
-def _on_device(first: torch.Tensor, *others) -> int:
-    """The device of all the tensors given: the current one, on whose stream
-    the call runs."""
-    device = first.get_device()
-    if device < 0 or device != _current_device():
-        raise ValueError("operands must be on the current GPU")
-    for t in others:
-        if t is not None and t.get_device() != device:
-            raise ValueError("operands must be on one GPU, the current one")
-    return device
+def _off_device():
+    raise ValueError("operands must be on one GPU, the current one")
 
 
 def _indices(t, name, count=None):
@@ -574,7 +566,7 @@ def _indices(t, name, count=None):
 
 
 def _floats(t, name, count):
-    if t.dtype != torch.float32 or not t.is_contiguous() or t.numel() != count:
+    if t.dtype != _f32 or not t.is_contiguous() or t.numel() != count:
         raise ValueError(f"{name} must be a dense f32 tensor of {count} values")
     return t
 
@@ -584,10 +576,10 @@ def _buffer(workspace, need, device, stream):
     made here is the allocator's again once the call returns: a stream other
     than the current one has to be known to it."""
     if workspace is not None:
+        if workspace.get_device() != _current_device():
+            _off_device()
         return workspace, workspace.data_ptr(), workspace.numel() * workspace.element_size()
-    if not need:
-        return None, None, 0
-    workspace = torch.empty(need, dtype=torch.uint8, device=device)
+    workspace = _empty(need, dtype=torch.uint8, device=device)
     if stream is not None:
         workspace.record_stream(stream if isinstance(stream, torch.cuda.Stream)
                                 else torch.cuda.ExternalStream(_stream(stream), device=device))
@@ -601,15 +593,20 @@ def group_rows(ids: torch.Tensor, groups: int, order=None, slots=None, offsets=N
     the shape of ids."""
     L = _lib or load()
     _indices(ids, "ids")
-    count = ids.numel()
-    order = torch.empty(count, dtype=_int32, device=ids.device) if order is None \
+    count, device = ids.numel(), ids.device
+    order = _empty(count, dtype=_int32, device=device) if order is None \
         else _indices(order, "order", count)
     slots = torch.empty_like(ids) if slots is None else _indices(slots, "slots", count)
-    offsets = torch.empty(groups + 1, dtype=_int32, device=ids.device) if offsets is None \
+    offsets = _empty(groups + 1, dtype=_int32, device=device) if offsets is None \
         else _indices(offsets, "offsets", groups + 1)
-    need = L.qlin_group_rows_workspace_bytes(count, groups) if count > 4096 else 0
-    workspace, ws_ptr, ws_bytes = _buffer(workspace, need, ids.device, stream)
-    _on_device(ids, order, slots, offsets, workspace)
+    d = ids.get_device()
+    if d < 0 or d != _current_device() or order.get_device() != d or slots.get_device() != d \
+            or offsets.get_device() != d:
+        _off_device()
+    ws_ptr, ws_bytes = None, 0
+    if count > 4096:
+        need = L.qlin_group_rows_workspace_bytes(count, groups)
+        workspace, ws_ptr, ws_bytes = _buffer(workspace, need, device, stream)
     _check(L.qlin_group_rows(ids.data_ptr(), count, groups, order.data_ptr(), slots.data_ptr(),
                              offsets.data_ptr(), ws_ptr, ws_bytes, _stream(stream)))
     return order, slots if slots.shape == ids.shape else slots.view(ids.shape), offsets
@@ -630,20 +627,24 @@ def route(logits: torch.Tensor, top_k: int, normalize: bool = False, ids=None, w
         raise ValueError("route expects 2-D f32/bf16/f16 logits with unit column stride")
     if tokens == 1 and ld < experts:
         ld = experts
-    count, device = tokens * top_k, logits.device
-    ids = torch.empty((tokens, top_k), dtype=_int32, device=device) if ids is None \
+    count, device, d = tokens * top_k, logits.device, logits.get_device()
+    ids = _empty((tokens, top_k), dtype=_int32, device=device) if ids is None \
         else _indices(ids, "ids", count)
-    weights = torch.empty((tokens, top_k), dtype=torch.float32, device=device) \
+    weights = _empty((tokens, top_k), dtype=_f32, device=device) \
         if weights is None else _floats(weights, "weights", count)
-    order = torch.empty(count, dtype=_int32, device=device) if order is None \
+    order = _empty(count, dtype=_int32, device=device) if order is None \
         else _indices(order, "order", count)
-    slots = torch.empty((tokens, top_k), dtype=_int32, device=device) if slots is None \
+    slots = _empty((tokens, top_k), dtype=_int32, device=device) if slots is None \
         else _indices(slots, "slots", count).view(tokens, top_k)
-    offsets = torch.empty(experts + 1, dtype=_int32, device=device) if offsets is None \
+    offsets = _empty(experts + 1, dtype=_int32, device=device) if offsets is None \
         else _indices(offsets, "offsets", experts + 1)
-    need = L.qlin_group_rows_workspace_bytes(count, experts) if count > 4096 else 0
-    workspace, ws_ptr, ws_bytes = _buffer(workspace, need, device, stream)
-    _on_device(logits, ids, weights, order, slots, offsets, workspace)
+    if d < 0 or d != _current_device() or ids.get_device() != d or weights.get_device() != d \
+            or order.get_device() != d or slots.get_device() != d or offsets.get_device() != d:
+        _off_device()
+    ws_ptr, ws_bytes = None, 0
+    if count > 4096:
+        need = L.qlin_group_rows_workspace_bytes(count, experts)
+        workspace, ws_ptr, ws_bytes = _buffer(workspace, need, device, stream)
     _check(L.qlin_route(logits.data_ptr(), ld, kind, tokens, experts, top_k, normalize,
                         ids.data_ptr(), weights.data_ptr(), order.data_ptr(), slots.data_ptr(),
                         offsets.data_ptr(), ws_ptr, ws_bytes, _stream(stream)))
@@ -656,25 +657,36 @@ def combine(h: torch.Tensor, slots: torch.Tensor, weights: torch.Tensor | None =
     slots int32 [tokens, top_k], weights f32 of the same shape (None = 1),
     base [tokens, N] or None. out may be base. Returns out [tokens, N]."""
     L = _lib or load()
-    kind = _TYPES.get(h.dtype)
+    dtype, d = h.dtype, h.get_device()
+    kind = _TYPES.get(dtype)
     if kind is None or h.dim() != 2 or not h.is_contiguous():
         raise ValueError("combine expects dense 2-D bf16/f16 rows")
-    if slots.dim() != 2:
-        raise ValueError("combine expects slots [tokens, top_k]")
-    _indices(slots, "slots")
+    if slots.dim() != 2 or slots.dtype != _int32 or not slots.is_contiguous():
+        raise ValueError("combine expects dense int32 slots [tokens, top_k]")
     tokens, top_k = slots.shape
     h_rows, N = h.shape
+    w_ptr = base_ptr = None
     if weights is not None:
         _floats(weights, "weights", tokens * top_k)
+        if weights.get_device() != d:
+            _off_device()
+        w_ptr = weights.data_ptr()
+    if base is not None:
+        if base.shape != (tokens, N) or base.dtype != dtype or not base.is_contiguous():
+            raise ValueError("combine base must be dense [tokens, N] in the rows' type")
+        if base.get_device() != d:
+            _off_device()
+        base_ptr = base.data_ptr()
+    if d < 0 or d != _current_device() or slots.get_device() != d:
+        _off_device()
     if out is None:
-        out = torch.empty((tokens, N), dtype=h.dtype, device=h.device)
-    for t in (base, out):
-        if t is not None and (t.shape != (tokens, N) or t.dtype != h.dtype
-                              or not t.is_contiguous()):
-            raise ValueError("combine base and output must be dense [tokens, N] in the rows' type")
-    _on_device(h, slots, weights, base, out)
-    _check(L.qlin_combine(h.data_ptr(), h_rows, slots.data_ptr(), _ptr(weights), _ptr(base),
-                          out.data_ptr(), tokens, top_k, N, kind, _stream(stream)))
+        out = _empty((tokens, N), dtype=dtype, device=h.device)
+    elif out.shape != (tokens, N) or out.dtype != dtype or not out.is_contiguous():
+        raise ValueError("combine output must be dense [tokens, N] in the rows' type")
+    elif out.get_device() != d:
+        _off_device()
+    _check(L.qlin_combine(h.data_ptr(), h_rows, slots.data_ptr(), w_ptr, base_ptr, out.data_ptr(),
+                          tokens, top_k, N, kind, _stream(stream)))
     return out
 
 
@@ -705,15 +717,22 @@ def expert_gemm(xq: torch.Tensor, sx: torch.Tensor, wq: torch.Tensor, sw: torch.
     _floats(sx, "expert_gemm row scales", blocks * x_rows)
     _floats(sw, "expert_gemm channel scales", experts * blocks * N)
     _indices(offsets, "offsets", experts + 1)
-    slots = x_rows if order is None else _indices(order, "order").numel()
+    d = xq.get_device()
+    slots, order_ptr = x_rows, None
+    if order is not None:
+        slots, order_ptr = _indices(order, "order").numel(), order.data_ptr()
+        if order.get_device() != d:
+            _off_device()
     if out is None:
-        out = torch.empty((slots, N), dtype=out_dtype, device=xq.device)
+        out = _empty((slots, N), dtype=out_dtype, device=xq.device)
     kind = _TYPES.get(out.dtype)
     if kind is None or out.shape != (slots, N) or not out.is_contiguous():
         raise ValueError("expert_gemm output must be dense bf16/f16 [slots, N]")
-    _on_device(xq, sx, wq, sw, offsets, order, out)
+    if d < 0 or d != _current_device() or sx.get_device() != d or wq.get_device() != d \
+            or sw.get_device() != d or offsets.get_device() != d or out.get_device() != d:
+        _off_device()
     _check(L.qlin_expert_gemm(None if path is None else ctypes.byref(path.to_c()), xq.data_ptr(),
-                              sx.data_ptr(), x_rows, _ptr(order), divisor, offsets.data_ptr(),
+                              sx.data_ptr(), x_rows, order_ptr, divisor, offsets.data_ptr(),
                               wq.data_ptr(), sw.data_ptr(), experts, out.data_ptr(), scatter, slots,
                               N, K, fmt, kind, group, _stream(stream)))
     return out
@@ -746,21 +765,33 @@ def adapter_add(x: torch.Tensor, order: torch.Tensor, offsets: torch.Tensor, a: 
         raise ValueError("adapter_add expects dense a [adapters, rank, K] and b [adapters, N, rank]")
     _indices(order, "order", rows)
     _indices(offsets, "offsets", adapters + 1)
-    base = y if base is None else base
+    d, shape = x.get_device(), (rows, N)
     ldx, ldy = (x.stride(0), y.stride(0)) if rows > 1 else (K, N)
-    for t in (y, base):
-        if t.shape != (rows, N) or t.dtype != dtype or (t.stride(1) != 1 and N > 1) \
-                or (rows > 1 and t.stride(0) != ldy):
-            raise ValueError("adapter_add base and output must be [rows, N] rows of one stride")
+    if y.shape != shape or y.dtype != dtype or (y.stride(1) != 1 and N > 1):
+        raise ValueError("adapter_add output must be [rows, N] rows in x's type")
+    if base is None:
+        base = y
+    elif base.shape != shape or base.dtype != dtype or (base.stride(1) != 1 and N > 1) \
+            or (rows > 1 and base.stride(0) != ldy) or base.get_device() != d:
+        raise ValueError("adapter_add base must be rows like the output's, of one stride")
+    ranks_ptr = scales_ptr = ws_ptr = None
     if ranks is not None:
-        _indices(ranks, "ranks", adapters)
+        ranks_ptr = _indices(ranks, "ranks", adapters).data_ptr()
+        if ranks.get_device() != d:
+            _off_device()
     if scales is not None:
-        _floats(scales, "scales", adapters)
-    need = 0 if workspace is not None else L.qlin_adapter_workspace_bytes(rows, adapters, K, rank)
-    workspace, ws_ptr, ws_bytes = _buffer(workspace, need, x.device, stream)
-    _on_device(x, order, offsets, a, b, y, base, ranks, scales, workspace)
+        scales_ptr = _floats(scales, "scales", adapters).data_ptr()
+        if scales.get_device() != d:
+            _off_device()
+    if d < 0 or d != _current_device() or order.get_device() != d or offsets.get_device() != d \
+            or a.get_device() != d or b.get_device() != d or y.get_device() != d:
+        _off_device()
+    # (The one-launch form needs none; only calls of many rows can take the other.)
+    ws_bytes = L.qlin_adapter_workspace_bytes(rows, adapters, K, rank) if rows * K > 1 << 17 else 0
+    if ws_bytes:
+        workspace, ws_ptr, ws_bytes = _buffer(workspace, ws_bytes, x.device, stream)
     _check(L.qlin_adapter_add(x.data_ptr(), ldx, order.data_ptr(), offsets.data_ptr(), rows, adapters,
-                              a.data_ptr(), b.data_ptr(), rank, _ptr(ranks), _ptr(scales),
+                              a.data_ptr(), b.data_ptr(), rank, ranks_ptr, scales_ptr,
                               base.data_ptr(), y.data_ptr(), ldy, N, K, kind, ws_ptr, ws_bytes,
                               _stream(stream)))
     return y
