@@ -548,7 +548,8 @@ def linear_noalloc(x: torch.Tensor, wq: torch.Tensor, sw: torch.Tensor, fmt: int
 # ---------------------------------------------------------------- rows grouped by weights
 # These run between the products of a decode step, where a call's time on the
 # host is what counts (of 7 us the launch is 3): checks read plain tensor
-# attributes, in line, and buffers are made in their final shape.
+# attributes, in line, and a call that makes its index arrays cuts them from one
+# allocation (an allocation is 1 to 1.4 us, a view 0.3).
 _LOGITS = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
 _int32, _f32 = torch.int32, torch.float32
 _empty, _current_device = torch.empty, torch.cuda.current_device
@@ -594,15 +595,20 @@ def group_rows(ids: torch.Tensor, groups: int, order=None, slots=None, offsets=N
     L = _lib or load()
     _indices(ids, "ids")
     count, device = ids.numel(), ids.device
-    order = _empty(count, dtype=_int32, device=device) if order is None \
-        else _indices(order, "order", count)
-    slots = torch.empty_like(ids) if slots is None else _indices(slots, "slots", count)
-    offsets = _empty(groups + 1, dtype=_int32, device=device) if offsets is None \
-        else _indices(offsets, "offsets", groups + 1)
     d = ids.get_device()
-    if d < 0 or d != _current_device() or order.get_device() != d or slots.get_device() != d \
-            or offsets.get_device() != d:
+    if d < 0 or d != _current_device():
         _off_device()
+    if order is None and slots is None and offsets is None and groups >= 0:
+        order, slots, offsets = _empty(2 * count + groups + 1, dtype=_int32, device=device) \
+            .split_with_sizes((count, count, groups + 1))
+    else:
+        order = _empty(count, dtype=_int32, device=device) if order is None \
+            else _indices(order, "order", count)
+        slots = torch.empty_like(ids) if slots is None else _indices(slots, "slots", count)
+        offsets = _empty(groups + 1, dtype=_int32, device=device) if offsets is None \
+            else _indices(offsets, "offsets", groups + 1)
+        if order.get_device() != d or slots.get_device() != d or offsets.get_device() != d:
+            _off_device()
     ws_ptr, ws_bytes = None, 0
     if count > 4096:
         need = L.qlin_group_rows_workspace_bytes(count, groups)
@@ -628,19 +634,29 @@ def route(logits: torch.Tensor, top_k: int, normalize: bool = False, ids=None, w
     if tokens == 1 and ld < experts:
         ld = experts
     count, device, d = tokens * top_k, logits.device, logits.get_device()
-    ids = _empty((tokens, top_k), dtype=_int32, device=device) if ids is None \
-        else _indices(ids, "ids", count)
-    weights = _empty((tokens, top_k), dtype=_f32, device=device) \
-        if weights is None else _floats(weights, "weights", count)
-    order = _empty(count, dtype=_int32, device=device) if order is None \
-        else _indices(order, "order", count)
-    slots = _empty((tokens, top_k), dtype=_int32, device=device) if slots is None \
-        else _indices(slots, "slots", count).view(tokens, top_k)
-    offsets = _empty(experts + 1, dtype=_int32, device=device) if offsets is None \
-        else _indices(offsets, "offsets", experts + 1)
-    if d < 0 or d != _current_device() or ids.get_device() != d or weights.get_device() != d \
-            or order.get_device() != d or slots.get_device() != d or offsets.get_device() != d:
+    if d < 0 or d != _current_device():
         _off_device()
+    if ids is None and weights is None and order is None and slots is None and offsets is None \
+            and count >= 0:
+        ids, weights, order, slots, offsets = \
+            _empty(4 * count + experts + 1, dtype=_int32, device=device) \
+            .split_with_sizes((count, count, count, count, experts + 1))
+        ids, slots = ids.view(tokens, top_k), slots.view(tokens, top_k)
+        weights = weights.view(_f32).view(tokens, top_k)
+    else:
+        ids = _empty((tokens, top_k), dtype=_int32, device=device) if ids is None \
+            else _indices(ids, "ids", count)
+        weights = _empty((tokens, top_k), dtype=_f32, device=device) \
+            if weights is None else _floats(weights, "weights", count)
+        order = _empty(count, dtype=_int32, device=device) if order is None \
+            else _indices(order, "order", count)
+        slots = _empty((tokens, top_k), dtype=_int32, device=device) if slots is None \
+            else _indices(slots, "slots", count).view(tokens, top_k)
+        offsets = _empty(experts + 1, dtype=_int32, device=device) if offsets is None \
+            else _indices(offsets, "offsets", experts + 1)
+        if ids.get_device() != d or weights.get_device() != d or order.get_device() != d \
+                or slots.get_device() != d or offsets.get_device() != d:
+            _off_device()
     ws_ptr, ws_bytes = None, 0
     if count > 4096:
         need = L.qlin_group_rows_workspace_bytes(count, experts)
@@ -680,7 +696,7 @@ def combine(h: torch.Tensor, slots: torch.Tensor, weights: torch.Tensor | None =
     if d < 0 or d != _current_device() or slots.get_device() != d:
         _off_device()
     if out is None:
-        out = _empty((tokens, N), dtype=dtype, device=h.device)
+        out = h.new_empty((tokens, N))
     elif out.shape != (tokens, N) or out.dtype != dtype or not out.is_contiguous():
         raise ValueError("combine output must be dense [tokens, N] in the rows' type")
     elif out.get_device() != d:
@@ -724,7 +740,7 @@ def expert_gemm(xq: torch.Tensor, sx: torch.Tensor, wq: torch.Tensor, sw: torch.
         if order.get_device() != d:
             _off_device()
     if out is None:
-        out = _empty((slots, N), dtype=out_dtype, device=xq.device)
+        out = xq.new_empty((slots, N), dtype=out_dtype)
     kind = _TYPES.get(out.dtype)
     if kind is None or out.shape != (slots, N) or not out.is_contiguous():
         raise ValueError("expert_gemm output must be dense bf16/f16 [slots, N]")
