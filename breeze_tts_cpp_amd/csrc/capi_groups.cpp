@@ -78,34 +78,40 @@ int check_grouping(const char *what, const int *ids, long count, int groups, con
 // The macro tile (index of kExpertTiles) for `slots` rows in `experts` groups,
 // of whose sizes the host knows no more than their mean. Measured with uneven
 // groups (weights from HBM, 80 shapes of 8-64 experts, 1024-4096 channels, K
-// 1024-4096, 0.25-1024 rows per expert, INT8 and group FP8):
+// 1024-4096, 0.25-1024 rows per expert, INT8 and FP8):
 //  - up to 8 rows per expert the weights' bytes are all: 64x32 tiles, two
 //    workgroups per CU (32 experts of 2048 x 2048, 4 rows each: 24.6 us, 26.7 with the
 //    K-sliced 32x16 tile). Where they would leave CUs without work, the K-sliced
 //    tile has twice the workgroups, each a quarter of the K walk (16 of 1024 x
-//    4096, 1 row: 10.2 us against 13.0; 8 of 64, 2048 x 2048: 8.4 against 8.9; with K
-//    groups only from K above 2048: 11.9 against 10.3 at 2048);
-//  - up to 96 rows 128x64 (16 rows: 27.7 us against 30.0 on 64x32, 31.3 on 256x128),
+//    4096, 1 row: 10.1 us against 13.0; 8 of 64, 2048 x 2048: 8.4 against 8.9; with K
+//    groups there 11.9 against 10.3, 2 of 8, 4096 x 2048, 7.3 against 9.2), with K above
+//    2048 up to 16 rows (16 of 1024 x 4096: 19.4 against 20.8 and 21.3);
+//  - up to 31 rows 128x64 (16 rows: 27.6 us against 29.8 on 64x32, 27.9 on 128x128),
 //    but 64x32 up to 32 rows where 128-channel tiles leave CUs without work (16 of
-//    1024 x 4096, 16 rows: 20.8 against 23.8);
-//  - above, the tile whose rounds of workgroups cost least, at the time that a
-//    round of each takes with uneven groups (128x64: two workgroups per CU), a part
-//    per 128 of K and a fixed one (prologue, epilogue). A 128x128 tile, two
-//    workgroups per CU, was best by at most 5%, for 128-256 rows of short K.
+//    1024 x 4096, 16 rows: 20.9 against 23.5), where also up to 96 rows 128x64 gives
+//    more of them some (64 rows: 24.6 against 26.9 on 128x128);
+//  - up to 127 rows 128x128 (64 rows: 36.7 us, 37.0 on 128x64, 48.6 on 256x256);
+//  - above, of 128x128 (two workgroups per CU) and 256x256 the tile whose rounds of
+//    workgroups cost least, at the time that a round of each takes with uneven
+//    groups, a part per 128 of K and a fixed one (prologue, epilogue).
 // With K groups 128x64 from 4 rows (6 rows, 31 experts of 2064 x 2048: 23.5 us, 26.7 on
-// 64x32), at any size (a 128x128 tile gains 15% at most, one round of long K).
-// On the 80 shapes the choice is within 7% of the best tile but for three (9-15%).
+// 64x32), at any size: the scales' arithmetic bounds it there, and a 128x128 tile is level
+// (125 rows, 64 experts of 2048 x 1024: 54-59 us in five forms against 56).
+// On the 80 shapes the choice is within 6% of the best tile.
 int choose_tile(long slots, int experts, int N, int K, int group) {
     const long each = slots / experts;
     const long some = slots < experts ? slots : experts;  // groups that can have rows
-    if (each <= 8 && some * ((N + 63) / 64) <= 256 && (!group || K > 2048)) return 0;
+    const bool few = some * ((N + 63) / 64) <= (group && K <= 2048 ? 128 : 256);
+    if (few && each <= (!group && K > 2048 ? 16 : 8)) return 0;
     if (each <= (group ? 3 : 8)) return 1;
-    if (each <= 32 && some * ((N + 127) / 128) < 256) return 1;
-    if (each <= 96 || group) return 2;
+    const bool idle = some * ((N + 127) / 128) < 256;  // CUs
+    if (each <= 32 && idle) return 1;
+    if (group || each < 32 || (each <= 96 && idle)) return 2;
+    if (each < 128) return 3;
     constexpr struct { int tile; long per_round; double stage, fixed; } kCost[] = {
-        {2, 512, 755, 3200}, {3, 256, 950, 7200}, {4, 256, 1765, 9500}};  // ns
+        {3, 512, 900, 6000}, {4, 256, 1350, 9000}};  // ns
     const double stages = double((long(K) + 127) / 128);
-    int best = 2;
+    int best = 3;
     double least = 1e300;
     for (const auto &c : kCost) {
         const auto &t = qlin::kExpertTiles[c.tile];

@@ -43,6 +43,7 @@ __device__ __forceinline__ void pin() {
     __builtin_amdgcn_sched_barrier(0);
 }
 
+// S = 2 (per-channel scales): a stage is refilled in halves (half_steps).
 template <int Fmt, bool Grouped, int KS, int WN, int WM, int NF, int MT, int S, int EU>
 __global__ __launch_bounds__(64 * KS * WN * WM, EU) void expert_gemm(ExpertArgs p, int tiles_n,
                                                                      int steps) {
@@ -214,12 +215,12 @@ __global__ __launch_bounds__(64 * KS * WN * WM, EU) void expert_gemm(ExpertArgs 
 #pragma unroll
         for (int t = 0; t < int(sizeof(b) / sizeof(b[0])); ++t) b[t] = frag(slot, BN + (t * WM + wm) * 16);
     };
-    auto read_w = [&](int slot, int f) { return frag(slot, (wn * NF + f) * 16); };
+    auto read_w = [&](int slot, int f) { return frag(slot, (f * WN + wn) * 16); };
     // The scales of a weight fragment's channels and of the wave's tokens.
     auto read_sw = [&](int slot, int f) {
         if constexpr (Grouped)
             return *reinterpret_cast<const f32x4 *>(ring + slot * STAGE + (BN + BM) * BK +
-                                                    ((wn * NF + f) * 16 + quad * 4) * 4);
+                                                    ((f * WN + wn) * 16 + quad * 4) * 4);
         else
             return f32x4{};
     };
@@ -255,9 +256,8 @@ __global__ __launch_bounds__(64 * KS * WN * WM, EU) void expert_gemm(ExpertArgs 
         static_for<0, XI>(dma_x);
         static_for<0, SI>(dma_s);
     }
-    static_assert(S == 2 || S == 3, "the waits below");
     int slot = 0;  // of the stage whose token fragments are in registers
-    // Step s: at its start every read of stage s - 1 has arrived (with a shared
+    // Step s of three stages: at its start every read of stage s - 1 has arrived (with a shared
     // ring in every wave), so that stage's slot takes stage s - 1 + S. Weight
     // fragments are read one 16-row block ahead of their MFMAs, the next stage's
     // token fragments and first weight fragment under the last block's, once
@@ -276,8 +276,8 @@ __global__ __launch_bounds__(64 * KS * WN * WM, EU) void expert_gemm(ExpertArgs 
         });
         slot = slot + 1 == S ? 0 : slot + 1;
         if (s + 1 < count) {  // stage s + 1, with at most one later one in flight
-            if (s == 0) wait_vmcnt<(XI + SI) * (S - 2)>();
-            else if (S == 3 && s + 2 < count) wait_vmcnt<INSTS>();
+            if (s == 0) wait_vmcnt<XI + SI>();
+            else if (s + 2 < count) wait_vmcnt<INSTS>();
             else wait_vmcnt<0>();
         }
         pin();
@@ -292,6 +292,55 @@ __global__ __launch_bounds__(64 * KS * WN * WM, EU) void expert_gemm(ExpertArgs 
         const f32x4 anw = read_sw(slot, 0);
         row(std::integral_constant<int, NF - 1>{}, a, aw, b, bx);
         a = an, aw = anw;
+    };
+    // Of two stages, refilled in halves: halfway through step s (at a barrier) every
+    // wave has read the stage's token rows and the first half of its weight rows, and
+    // stage s + 2's take their place; at its end the other half. So a whole stage
+    // is in flight at every wait, with 1.5 steps to arrive in. Refilled as a whole,
+    // none was (4096 tokens x 4 of 32 experts, 4096 x 2048, 256x256 tiles: INT8 187 -> 170
+    // us, FP8 178 -> 160; with three stages of weight rows 174, 165). Stages past the
+    // walk's end load as zeros, so that the counts hold.
+    constexpr int WL = WI / 2, HALF = NF / 2;
+    static_assert(S == 3 || (S == 2 && !Grouped && NWS > 1 && WI % 2 == 0 && NF % 2 == 0), "the steps");
+    auto half_steps = [&](int s, i32x8 &a, const auto &b, auto &nb) {
+        if (s > 0) {
+            aim(s + 1, slot ^ 1);
+            static_for<WL, WI>(dma_w);
+        }
+        static_for<0, NF - 1>([&](auto f_) {
+            constexpr int f = decltype(f_)::value;
+            if constexpr (f == HALF - 1) {
+                wait_vmcnt<INSTS>();  // this stage's second half has landed
+                pin();
+                wait_lds_reads();
+                __builtin_amdgcn_s_barrier();
+                pin();
+            }
+            const i32x8 an = read_w(slot, f + 1);
+            if constexpr (f == HALF - 1) {
+                aim(s + 2, slot);
+                static_for<0, WL>(dma_w);
+                static_for<0, XI>(dma_x);
+            }
+            row(f_, a, f32x4{}, b, 0);
+            a = an;
+            pin();
+        });
+        slot ^= 1;
+        if (s == 0) wait_vmcnt<WL + XI>();  // stage s + 1's token rows and first half
+        else wait_vmcnt<INSTS>();
+        pin();
+        wait_lds_reads();
+        __builtin_amdgcn_s_barrier();
+        pin();
+        read_x(slot, nb);
+        const i32x8 an = read_w(slot, 0);
+        row(std::integral_constant<int, NF - 1>{}, a, f32x4{}, b, 0);
+        a = an;
+    };
+    auto any_step = [&](int s, i32x8 &a, f32x4 &aw, const auto &b, const auto &bx, auto &nb, auto &nbx) {
+        if constexpr (S == 2) half_steps(s, a, b, nb);
+        else step(s, a, aw, b, bx, nb, nbx);
     };
     // All stages for the wave's first L token fragments.
     auto walk = [&](auto live_) {
@@ -308,10 +357,10 @@ __global__ __launch_bounds__(64 * KS * WN * WM, EU) void expert_gemm(ExpertArgs 
         aw = read_sw(0, 0);
         int s = 0;
         for (; s + 1 < count; s += 2) {
-            step(s, a, aw, b0, x0, b1, x1);
-            step(s + 1, a, aw, b1, x1, b0, x0);
+            any_step(s, a, aw, b0, x0, b1, x1);
+            any_step(s + 1, a, aw, b1, x1, b0, x0);
         }
-        if (s < count) step(s, a, aw, b0, x0, b1, x1);
+        if (s < count) any_step(s, a, aw, b0, x0, b1, x1);
     };
     // The waves along the tokens take the tile's 16-row fragments in turn, so a
     // group's short last tile has fewer in every wave, and only those are
@@ -355,7 +404,7 @@ __global__ __launch_bounds__(64 * KS * WN * WM, EU) void expert_gemm(ExpertArgs 
             const float scale_x = row_scale[ml];
 #pragma unroll
             for (int f = 0; f < NF; ++f) {
-                const int nl = (wn * NF + f) * 16 + quad * 4;
+                const int nl = (f * WN + wn) * 16 + quad * 4;
                 float v[4];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
@@ -396,7 +445,7 @@ __global__ __launch_bounds__(64 * KS * WN * WM, EU) void expert_gemm(ExpertArgs 
 #pragma unroll
             for (int f = 0; f < NF; ++f)
                 *reinterpret_cast<Red4 *>(red + (ks * BM + (t * WM + wm) * 16 + row16) * PITCH +
-                                          (wn * NF + f) * 16 + quad * 4) = acc[f][t];
+                                          (f * WN + wn) * 16 + quad * 4) = acc[f][t];
         __syncthreads();
         const int nl = tid % (BN / 4) * 4, r0 = tid / (BN / 4);
         if (n_base + nl >= N || r0 >= kPass) return;

@@ -196,7 +196,7 @@ struct ExpertArgs {
     X(1, 1, 4, 1, 1, 2, 3, 4) \
     X(2, 1, 4, 2, 2, 2, 3, 4)
 #define QLIN_EXPERT_WIDE_TILES(X) \
-    X(3, 1, 4, 2, 4, 4, 3, 2)     \
+    X(3, 1, 4, 2, 2, 4, 2, 4)     \
     X(4, 1, 2, 4, 8, 4, 2, 2)
 constexpr int kExpertNarrowTiles = 3;
 struct ExpertTile {

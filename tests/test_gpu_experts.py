@@ -93,6 +93,35 @@ def test_every_tile(dev, N, K):
         run_case(dev, mode, SIZES, N, K, top_k=3, path=path, absent=9)
 
 
+@pytest.mark.parametrize("K", [256, 384, 528])
+def test_every_tile_whole(dev, K):
+    """Whole and nearly whole tiles, few stages of K."""
+    for mode, path in every_path():
+        run_case(dev, mode, [256, 0, 257, 193], 272, K, top_k=2, path=path)
+
+
+@pytest.mark.parametrize("mode", MODES)
+def test_every_tile_repeats(dev, mode):
+    """The same call gives the same bits, with every CU at work."""
+    from breeze_tts_cpp_amd import qlinear
+    g = torch.Generator().manual_seed(17)
+    fmt, group = MODES[mode]
+    count, experts, N, K = 3000, 8, 1040, 1680
+    ids = torch.randint(0, experts, (count,), generator=g, dtype=torch.int32).to(dev)
+    x, sx = codes(g, count, K, mode)
+    w, sw = codes(g, N, K, mode)
+    x, sx, w = x.to(dev), sx.to(dev), torch.stack([w] * experts).to(dev)
+    sw = torch.stack([sw] * experts).to(dev)
+    order, _, offsets = qlinear.group_rows(ids, experts)
+    for path in [p for m, p in every_path() if m == mode]:
+        first = None
+        for _ in range(6):
+            out = qlinear.expert_gemm(x, sx, w, sw, fmt, offsets, order=order, scatter=True,
+                                      group=group, path=path)
+            first = out if first is None else first
+            assert torch.equal(out, first), path
+
+
 @pytest.mark.parametrize("mode", MODES)
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
 @pytest.mark.parametrize("gather,scatter", [(False, False), (True, False), (True, True)])
