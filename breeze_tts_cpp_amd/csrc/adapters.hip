@@ -193,25 +193,36 @@ __device__ __forceinline__ void split_token(const float (&t)[RP / 16], uint16_t 
 }
 
 constexpr int rank_pad(int rt) { return rt < 2 ? 32 : 16 * rt; }
+// Floats between two tokens of the waves' partial t: 16 tokens of a write on
+// distinct banks (4096 rows of rank 64, 2048 x 6144: 38.5 -> 37.1 us).
+constexpr int part_pitch(int rt) { return rank_pad(rt) + 4; }
 constexpr int kAdapterWaves = 8, kAdapterThreads = 64 * kAdapterWaves;
 constexpr int kPassChannels = 32 * kAdapterWaves;  // of the second product at a time
 constexpr int kDeltaPitch = kPassChannels + 4;     // floats
 
-// Two buffers of a pass's results (one serves a single pass).
-constexpr int results_bytes(int mt, bool one_pass = false) {
-    return (one_pass ? 1 : 2) * 16 * mt * kDeltaPitch * 4;
+// Two buffers of a pass's results.
+constexpr int results_bytes(int mt) { return 2 * 16 * mt * kDeltaPitch * 4; }
+// A single pass (Once) puts a wave's results, 32 channels of each token, where its
+// B panel was, so that a CU takes three workgroups up to rank 64 (4096 rows of rank 64:
+// 2048 x 6144 37.1 -> 35.2 us, 6144 x 2048 57 -> 46; of rank 128, with LDS for one, 39.4 ->
+// 44.6: there a workgroup runs its passes in turn). Two lanes at most meet in a bank.
+constexpr int kOncePitch = 36;  // floats
+constexpr int once_bytes(int rp, int mt) {
+    const int panel = 32 * rp * 2, results = 16 * mt * kOncePitch * 4;
+    return (panel > results ? panel : results) + 128;
 }
 
 // The second product of the tile's 16 MT tokens for channels [n_begin, n_end), 256 at a time,
 // 32 a wave: B's rows (one contiguous block of memory) through LDS like the
 // operands above, the results through LDS to whole row pieces, so that base and y
 // move in runs of 512 bytes. t is in hi / lo [16 MT][RP + 8]; `panel` holds 32 rows of B a
-// wave, `results` two buffers of a pass's fp32 results.
-template <class T, int RP, int MT, bool VecB, bool VecY> struct Expand {
+// wave, `results` two buffers of a pass's fp32 results (Once: not used).
+template <class T, int RP, int MT, bool VecB, bool VecY, bool Once> struct Expand {
     // Rows of RP * 2 bytes, chunk c of row r at c ^ swizzle(r): fragment reads on
     // distinct banks. Chunks past the rank arrive as zeros; one that holds the
     // rank's end is cut when it is read.
     static constexpr int kChunks = RP / 8, kPanel = 32 * RP * 2;
+    static constexpr int kStep = Once ? once_bytes(RP, MT) : kPanel;  // of the waves' LDS
     const AdapterArgs &p;
     const RowTile &tile;
     int rank, n_begin, n_end;
@@ -222,7 +233,7 @@ template <class T, int RP, int MT, bool VecB, bool VecY> struct Expand {
                                       uint8_t *panels)
         : p(p_), tile(tile_), rank(rank_), n_begin(tile_.column * width),
           n_end(min(tile_.column * width + width, p_.N)),
-          panel(panels + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * kPanel),
+          panel(panels + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * kStep),
           to_column(threadIdx.x % 32 * 8) {
 #pragma unroll
         for (int t = 0; t < MT; ++t) to_row[t] = source_row(p, tile, t * 16 + int(threadIdx.x) / 32);
@@ -304,11 +315,14 @@ template <class T, int RP, int MT, bool VecB, bool VecY> struct Expand {
             wait_lds_reads();
             pin();
             cut(bv);
-            if (n0 + kPassChannels < n_end) {
+            if (!Once && n0 + kPassChannels < n_end) {
                 issue(n0 + kPassChannels);
                 load_base(n0 + kPassChannels, next);
             }
-            float *at = results + half * 16 * MT * kDeltaPitch;
+            // [token][channel of the pass or, once, of the wave]
+            float *at = Once ? reinterpret_cast<float *>(panel)
+                             : results + half * 16 * MT * kDeltaPitch + wave * 32;
+            constexpr int kPitchOut = Once ? kOncePitch : kDeltaPitch;
 #pragma unroll
             for (int t = 0; t < MT; ++t) {
                 f32x4 out[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
@@ -327,7 +341,7 @@ template <class T, int RP, int MT, bool VecB, bool VecY> struct Expand {
                 for (int f = 0; f < 2; ++f) {
 #pragma unroll
                     for (int r = 0; r < 4; ++r) out[f][r] = scale * __builtin_amdgcn_ldexpf(out[f][r], e);
-                    *reinterpret_cast<f32x4 *>(at + ml * kDeltaPitch + wave * 32 + quad * 8 + f * 4) = out[f];
+                    *reinterpret_cast<f32x4 *>(at + ml * kPitchOut + quad * 8 + f * 4) = out[f];
                 }
             }
             lds_barrier();  // (the other half was read before the last one)
@@ -335,7 +349,10 @@ template <class T, int RP, int MT, bool VecB, bool VecY> struct Expand {
 #pragma unroll
             for (int t = 0; t < MT; ++t) {
                 if (to_row[t] < 0 || n >= n_end) continue;
-                const float *delta = at + (t * 16 + threadIdx.x / 32) * kDeltaPitch + to_column;
+                const int ml = t * 16 + threadIdx.x / 32;
+                const uint8_t *other = panel + (to_column / 32 - wave) * kStep;  // of the channels' wave
+                const float *delta = Once ? reinterpret_cast<const float *>(other) + ml * kPitchOut + to_column % 32
+                                          : at - wave * 32 + ml * kPitchOut + to_column;
                 float v[8];
                 widen8<T>(base[t], v);
 #pragma unroll
@@ -344,6 +361,7 @@ template <class T, int RP, int MT, bool VecB, bool VecY> struct Expand {
             }
 #pragma unroll
             for (int t = 0; t < MT; ++t) base[t] = next[t];
+            if constexpr (Once) break;
         }
     }
 };
@@ -358,7 +376,7 @@ struct AdapterLds {
 constexpr AdapterLds adapter_lds(int rt) {
     AdapterLds l{};
     l.stage = 16 * (rt + 1) * 128;
-    const int sums = kAdapterWaves * 16 * rank_pad(rt) * 4, results = results_bytes(1);
+    const int sums = kAdapterWaves * 16 * part_pitch(rt) * 4, results = results_bytes(1);
     const int reused = sums > results ? sums : results;
     const int stages = kAdapterWaves * l.stage;
     l.panels_at = rt == 8 || reused > stages ? reused : stages;
@@ -383,7 +401,7 @@ __global__ __launch_bounds__(kAdapterThreads) void adapter_rows(AdapterArgs p, i
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int rank = group_rank(p, tile.group);
     const int rows[2] = {source_row(p, tile, lane >> 3), source_row(p, tile, 8 + (lane >> 3))};
-    const Expand<T, RP, 1, VecB, VecY> second(p, tile, rank, width, lds + kLds.panels_at);
+    const Expand<T, RP, 1, VecB, VecY, false> second(p, tile, rank, width, lds + kLds.panels_at);
     pin();
     if constexpr (RT < 8) second.issue(second.n_begin);
 
@@ -398,7 +416,7 @@ __global__ __launch_bounds__(kAdapterThreads) void adapter_rows(AdapterArgs p, i
     if constexpr (RT == 8) second.issue(second.n_begin);
 #pragma unroll
     for (int i = 0; i < RP / 16; ++i)
-        *reinterpret_cast<f32x4 *>(parts + (wave * 16 + row16) * RP + i * 16 + quad * 4) =
+        *reinterpret_cast<f32x4 *>(parts + (wave * 16 + row16) * part_pitch(RT) + i * 16 + quad * 4) =
             i < RT ? acc[i < RT ? i : 0][0] : f32x4{0, 0, 0, 0};
     __syncthreads();
     if (threadIdx.x < 256) {  // 16 lanes per token
@@ -408,7 +426,7 @@ __global__ __launch_bounds__(kAdapterThreads) void adapter_rows(AdapterArgs p, i
         for (int i = 0; i < RP / 16; ++i) {
             t[i] = 0.f;
 #pragma unroll
-            for (int q = 0; q < W; ++q) t[i] += parts[(q * 16 + ml) * RP + i * 16 + l];
+            for (int q = 0; q < W; ++q) t[i] += parts[(q * 16 + ml) * part_pitch(RT) + i * 16 + l];
             // (Past the rank A was read as zeros, but 0 * inf is NaN.)
             if (i * 16 + l >= rank) t[i] = 0.f;
         }
@@ -424,7 +442,7 @@ __global__ __launch_bounds__(kAdapterThreads) void adapter_rows(AdapterArgs p, i
 constexpr int kShrinkRows = 64, kExpandRows = 32, kShrinkWaves = 4, kMaxSplits = 4;
 constexpr int shrink_lds_bytes(int rt) {
     const int rts = rt < 4 ? rt : 4, rings = kShrinkWaves * 2 * 16 * (rts + kShrinkRows / 16) * 128;
-    const int sums = kShrinkWaves * kShrinkRows * rank_pad(rts) * 4;
+    const int sums = kShrinkWaves * kShrinkRows * part_pitch(rts) * 4;
     return rings > sums ? rings : sums;
 }
 // First product of a 64-row tile over one of `splits` ranges of K, which its four
@@ -460,13 +478,14 @@ __global__ __launch_bounds__(64 * kShrinkWaves) void adapter_shrink(AdapterArgs 
     for (int t = 0; t < MT; ++t)
 #pragma unroll
         for (int i = 0; i < RPS / 16; ++i)
-            *reinterpret_cast<f32x4 *>(parts + ((wave * MT + t) * 16 + row16) * RPS + i * 16 + quad * 4) =
+            *reinterpret_cast<f32x4 *>(parts + ((wave * MT + t) * 16 + row16) * part_pitch(RTS) + i * 16 + quad * 4) =
                 i < RTS ? acc[i < RTS ? i : 0][t] : f32x4{0, 0, 0, 0};
     __syncthreads();
     for (int i = threadIdx.x * 4; i < tile.rows * RPS; i += 64 * W * 4) {
         f32x4 s = f32x4{0, 0, 0, 0};
 #pragma unroll
-        for (int q = 0; q < W; ++q) s += *reinterpret_cast<const f32x4 *>(parts + q * 16 * MT * RPS + i);
+        for (int q = 0; q < W; ++q)
+            s += *reinterpret_cast<const f32x4 *>(parts + (q * 16 * MT + i / RPS) * part_pitch(RTS) + i % RPS);
         *reinterpret_cast<f32x4 *>(out + size_t(i / RPS) * RP + i % RPS) = s;
     }
 }
@@ -476,13 +495,14 @@ template <class T, int RT, bool VecB, bool VecY>
 __global__ __launch_bounds__(kAdapterThreads) void adapter_expand(AdapterArgs p, int splits, int columns,
                                                                   int width) {
     constexpr int RP = rank_pad(RT), MT = kExpandRows / 16, kPitch = RP + 8;
+    constexpr bool kOnce = RT <= 4;
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
     __shared__ __attribute__((aligned(16))) uint16_t hi[16 * MT * kPitch], lo[16 * MT * kPitch];
     __shared__ int exponent[16 * MT];
     RowTile tile;
     if (!find_tile(p.offsets, p.adapters, p.rows, 16 * MT, columns, blockIdx.x, tile)) return;
     const int rank = group_rank(p, tile.group);
-    const Expand<T, RP, MT, VecB, VecY> second(p, tile, rank, width, lds);
+    const Expand<T, RP, MT, VecB, VecY, kOnce> second(p, tile, rank, width, lds);
     second.issue(second.n_begin);
     uint4 base[MT];
     second.load_base(second.n_begin, base);
@@ -507,15 +527,19 @@ __global__ __launch_bounds__(kAdapterThreads) void adapter_expand(AdapterArgs p,
     second.run(hi, lo, exponent, reinterpret_cast<float *>(lds + kAdapterWaves * 32 * RP * 2), base);
 }
 
-// Splits of K of the two-launch form; 0: one launch, while the A matrices that its 16-row
-// tiles read come to less than 64 MB (one / two launches, us: 1000 rows of rank 64,
-// 12288 x 2048, 17 MB, 25.6 / 27.2; 4096 rows of 2048 x 6144: rank 16, 51 MB, 26 / 28,
-// rank 32 34 / 26, rank 64 45 / 31.5, rank 128 73 / 53). The 64-row tiles times the
-// splits make one round of workgroups: in a second one 4096 rows of rank 64 take 44.
+// Splits of K of the two-launch form; 0: one launch, while the A matrices that its
+// 16-row tiles read come to less than 32 MiB (rank 16: 48 MiB). One / two launches, us:
+// 500 rows of 100 adapters of rank 64, 4096 x 2048, 31 MiB, 22.8 / 28.1; 1000 of 64 of rank
+// 32, 4096 x 4096, 30 MiB, 15.6 / 17.9; 2048 of 8 of rank 32, 4096 x 4096, 34 MiB, 25.6 /
+// 19.6; 4096 of 6 of rank 64, 6144 x 2048, 65 MiB, 72 / 43; rank 16: 8192 of 8, 2048 x 2048,
+// 32 MiB, 24.6 / 30.0, 4096 of 6, 2048 x 6144, 49 MiB, 32.6 / 24.3. The 64-row tiles times
+// the splits make one round of workgroups: in a second one 4096 rows of rank 64 take 44 us
+// in place of 35 (two smaller workgroups per CU, 512 in a round, 38-40), of rank 128, 2048 x
+// 2048, 40 in place of 37.
 int plan_splits(int rows, int adapters, int K, int rank) {
-    if (expert_row_tiles(rows, adapters, 16) * rank * K * 2 < 64L << 20) return 0;
-    const long tiles = expert_row_tiles(rows, adapters, kShrinkRows);
-    return int(std::max(1L, std::min(std::min(256 / tiles, long(kMaxSplits)), long(K) / 512)));
+    if (expert_row_tiles(rows, adapters, 16) * rank * K * 2 < (rank <= 16 ? 48L : 32L) << 20) return 0;
+    const long groups = expert_row_tiles(rows, adapters, kShrinkRows) * (rank > 64 ? 2 : 1);
+    return int(std::max(1L, std::min(std::min(256 / groups, long(kMaxSplits)), long(K) / 512)));
 }
 
 template <class T, int RT, bool VecX, bool VecB, bool VecY>
@@ -531,12 +555,13 @@ void launch_as(const AdapterArgs &a, hipStream_t s) {
         hipLaunchKernelGGL((adapter_shrink<T, RT, VecX>), dim3(unsigned(tiles * splits * (RT > 4 ? 2 : 1))),
                            dim3(64 * kShrinkWaves), shrink_lds_bytes(RT), s, a, splits);
         const long rows = expert_row_tiles(a.rows, a.adapters, kExpandRows);
-        const int width = width_of(rows, RT == 8 ? 1024 : 2048), columns = (a.N + width - 1) / width;
-        constexpr int kPanels = kAdapterWaves * 32 * rank_pad(RT) * 2;
-        static_assert(kPanels + results_bytes(2) + 4 * kExpandRows * (rank_pad(RT) + 9) <= int(kLdsBytes), "LDS");
-        const int bytes = kPanels + results_bytes(kExpandRows / 16, width == kPassChannels);
-        hipLaunchKernelGGL((adapter_expand<T, RT, VecB, VecY>), dim3(unsigned(rows * columns)),
-                           dim3(kAdapterThreads), bytes, s, a, splits, columns, width);
+        const int width = RT <= 4 ? kPassChannels : width_of(rows, 1024), columns = (a.N + width - 1) / width;
+        constexpr int RP = rank_pad(RT), MT = kExpandRows / 16;
+        constexpr int bytes = kAdapterWaves * (RT <= 4 ? once_bytes(RP, MT) : 32 * RP * 2) +
+                              (RT <= 4 ? 0 : results_bytes(MT));
+        static_assert(bytes + 4 * kExpandRows * (RP + 9) <= int(kLdsBytes), "LDS");
+        hipLaunchKernelGGL((adapter_expand<T, RT, VecB, VecY>), dim3(unsigned(rows * columns)), dim3(kAdapterThreads),
+                           bytes, s, a, splits, columns, width);
         return;
     }
     // Column tiles until the workgroups fill the CUs; of ranks up to 32, whose

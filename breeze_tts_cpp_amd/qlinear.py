@@ -803,7 +803,7 @@ def adapter_add(x: torch.Tensor, order: torch.Tensor, offsets: torch.Tensor, a: 
             or a.get_device() != d or b.get_device() != d or y.get_device() != d:
         _off_device()
     # (The one-launch form needs none; only calls of many rows can take the other.)
-    ws_bytes = L.qlin_adapter_workspace_bytes(rows, adapters, K, rank) if rows * K > 1 << 17 else 0
+    ws_bytes = L.qlin_adapter_workspace_bytes(rows, adapters, K, rank) if rows * K >= 1 << 17 else 0
     if ws_bytes:
         workspace, ws_ptr, ws_bytes = _buffer(workspace, ws_bytes, x.device, stream)
     _check(L.qlin_adapter_add(x.data_ptr(), ldx, order.data_ptr(), offsets.data_ptr(), rows, adapters,
