@@ -95,8 +95,8 @@ int check_grouping(const char *what, const int *ids, long count, int groups, con
 //    workgroups cost least, at the time that a round of each takes with uneven
 //    groups, a part per 128 of K and a fixed one (prologue, epilogue).
 // With K groups 128x64 from 4 rows (6 rows, 31 experts of 2064 x 2048: 23.5 us, 26.7 on
-// 64x32), at any size: the scales' arithmetic bounds it there, and a 128x128 tile is level
-// (125 rows, 64 experts of 2048 x 1024: 54-59 us in five forms against 56).
+// 64x32), at any size: beside the scales' registers a 128x128 tile is level (125 rows, 64
+// experts of 2048 x 1024: 54-59 us in five forms against 56).
 // On the 80 shapes the choice is within 6% of the best tile.
 int choose_tile(long slots, int experts, int N, int K, int group) {
     const long each = slots / experts;
