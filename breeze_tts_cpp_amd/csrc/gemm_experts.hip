@@ -14,7 +14,7 @@
 // arrive as zeros (out-of-range offsets). The partial tiles of the slices are
 // summed through LDS in ascending slice order.
 //
-// Bound by the live experts' weights while an expert has few rows (96 slots of 64
+// Bound by the live experts' weights while an expert has few rows (192 slots of 64
 // experts, 2048 x 1024 FP8: 20.9 us, 5.3 TB/s with what the Infinity Cache gives; 8 of 64, 2048 x
 // 2048 INT8: 7.6 us, 4.4 TB/s), by the MFMAs and short last tiles with many (16384 slots of 32
 // experts, 4096 x 2048 INT8: 158 us, 1.74 POPS; 4096 rows each 2.0), between them
