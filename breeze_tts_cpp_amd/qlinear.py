@@ -553,6 +553,7 @@ def linear_noalloc(x: torch.Tensor, wq: torch.Tensor, sw: torch.Tensor, fmt: int
 _LOGITS = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
 _int32, _f32 = torch.int32, torch.float32
 _empty, _current_device = torch.empty, torch.cuda.current_device
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # (None in a build without GPUs)
 
 
 def _off_device():
@@ -614,7 +615,8 @@ def group_rows(ids: torch.Tensor, groups: int, order=None, slots=None, offsets=N
         need = L.qlin_group_rows_workspace_bytes(count, groups)
         workspace, ws_ptr, ws_bytes = _buffer(workspace, need, device, stream)
     _check(L.qlin_group_rows(ids.data_ptr(), count, groups, order.data_ptr(), slots.data_ptr(),
-                             offsets.data_ptr(), ws_ptr, ws_bytes, _stream(stream)))
+                             offsets.data_ptr(), ws_ptr, ws_bytes,
+                             _raw_stream(d) if stream is None else _stream(stream)))
     return order, slots if slots.shape == ids.shape else slots.view(ids.shape), offsets
 
 
@@ -663,7 +665,8 @@ def route(logits: torch.Tensor, top_k: int, normalize: bool = False, ids=None, w
         workspace, ws_ptr, ws_bytes = _buffer(workspace, need, device, stream)
     _check(L.qlin_route(logits.data_ptr(), ld, kind, tokens, experts, top_k, normalize,
                         ids.data_ptr(), weights.data_ptr(), order.data_ptr(), slots.data_ptr(),
-                        offsets.data_ptr(), ws_ptr, ws_bytes, _stream(stream)))
+                        offsets.data_ptr(), ws_ptr, ws_bytes,
+                        _raw_stream(d) if stream is None else _stream(stream)))
     return ids, weights, order, slots, offsets
 
 
@@ -702,7 +705,8 @@ def combine(h: torch.Tensor, slots: torch.Tensor, weights: torch.Tensor | None =
     elif out.get_device() != d:
         _off_device()
     _check(L.qlin_combine(h.data_ptr(), h_rows, slots.data_ptr(), w_ptr, base_ptr, out.data_ptr(),
-                          tokens, top_k, N, kind, _stream(stream)))
+                          tokens, top_k, N, kind,
+                          _raw_stream(d) if stream is None else _stream(stream)))
     return out
 
 
@@ -750,7 +754,8 @@ def expert_gemm(xq: torch.Tensor, sx: torch.Tensor, wq: torch.Tensor, sw: torch.
     _check(L.qlin_expert_gemm(None if path is None else ctypes.byref(path.to_c()), xq.data_ptr(),
                               sx.data_ptr(), x_rows, order_ptr, divisor, offsets.data_ptr(),
                               wq.data_ptr(), sw.data_ptr(), experts, out.data_ptr(), scatter, slots,
-                              N, K, fmt, kind, group, _stream(stream)))
+                              N, K, fmt, kind, group,
+                              _raw_stream(d) if stream is None else _stream(stream)))
     return out
 
 
@@ -809,5 +814,5 @@ def adapter_add(x: torch.Tensor, order: torch.Tensor, offsets: torch.Tensor, a: 
     _check(L.qlin_adapter_add(x.data_ptr(), ldx, order.data_ptr(), offsets.data_ptr(), rows, adapters,
                               a.data_ptr(), b.data_ptr(), rank, ranks_ptr, scales_ptr,
                               base.data_ptr(), y.data_ptr(), ldy, N, K, kind, ws_ptr, ws_bytes,
-                              _stream(stream)))
+                              _raw_stream(d) if stream is None else _stream(stream)))
     return y
