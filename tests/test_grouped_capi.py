@@ -172,3 +172,13 @@ def test_binding_refusals():
         qlinear.adapter_add(xb, order[:3], offsets, a, b, y)
     with pytest.raises(ValueError):
         qlinear.adapter_add(xb, order, offsets, a, b, y, base=torch.zeros(4, 32, dtype=torch.bfloat16)[:, :16])
+
+
+def test_small_adapter_calls_need_no_workspace():
+    """The bound below which the binding does not ask: no adapter count or rank needs one there."""
+    for rows in (1, 15, 16, 64, 511, 1000, 4096):
+        K = ((1 << 17) - 1) // rows // 16 * 16
+        for adapters in (1, 2, rows, 1024):
+            for rank in (1, 16, 17, 32, 64, 65, 128):
+                assert K < 16 or qlinear.adapter_workspace_bytes(rows, adapters, K, rank) == 0
+    assert qlinear.adapter_workspace_bytes(64, 64, 2048, 128) > 0
