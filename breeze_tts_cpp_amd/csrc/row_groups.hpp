@@ -22,6 +22,18 @@ __device__ __forceinline__ int wave_scan(int v) {
     return v;
 }
 
+// The same with the maximum in place of the sum (values from 0 on; unsigned, so that
+// the exchange folds into the maximum).
+__device__ __forceinline__ int wave_scan_max(uint32_t v) {
+    v = max(v, uint32_t(__builtin_amdgcn_update_dpp(0, int(v), 0x111, 0xF, 0xF, true)));
+    v = max(v, uint32_t(__builtin_amdgcn_update_dpp(0, int(v), 0x112, 0xF, 0xF, true)));
+    v = max(v, uint32_t(__builtin_amdgcn_update_dpp(0, int(v), 0x114, 0xF, 0xF, true)));
+    v = max(v, uint32_t(__builtin_amdgcn_update_dpp(0, int(v), 0x118, 0xF, 0xF, true)));
+    v = max(v, uint32_t(__builtin_amdgcn_update_dpp(0, int(v), 0x142, 0xA, 0xF, false)));
+    v = max(v, uint32_t(__builtin_amdgcn_update_dpp(0, int(v), 0x143, 0xC, 0xF, false)));
+    return int(v);
+}
+
 // One tile of a grouped product: `rows` slots from `begin` of group `group`,
 // column tile `column`.
 struct RowTile {
@@ -34,23 +46,28 @@ struct RowTile {
 // hardware places workgroup i on XCD i % 8: every 256 workgroups (a round of the
 // CUs) take 256 tiles, each XCD 32 in a run that share its L2; the rest of the
 // tiles is numbered XCD-major. (All tiles XCD-major puts whole groups on one XCD,
-// and groups differ in size: a 4096-token prefill over 32 experts 5% slower.) False past the last tile. Offsets are held to [0, slots] and
-// ascending order here, so bad ones cannot lead out of the arrays. Same
-// result in every lane of the workgroup.
+// and groups differ in size: a 4096-token prefill over 32 experts 5% slower.) False past the last tile.
+// Bad offsets cannot lead out of the arrays, nor two groups to one slot: each is
+// held to [0, slots] and to the largest before it, so that a slot belongs to the
+// first group that claims it and the tiles are no more than the launch's bound.
+// Same result in every lane of the workgroup.
 __device__ __forceinline__ bool find_tile(const int *__restrict__ offsets, int groups, int slots,
                                           int height, int columns, int index, RowTile &tile) {
     const int lane = threadIdx.x & 63;
-    auto load = [&](int g, int &begin) {
-        begin = min(max(offsets[min(g, groups)], 0), slots);
-        const int end = min(offsets[min(g + 1, groups)], slots);
-        return max(end - begin, 0);
+    // Rows of the groups [g0, g0 + 64), one a lane, after offsets up to `largest`.
+    auto load = [&](int g0, int &largest, int &begin) {
+        const int g = g0 + lane;
+        const int from = offsets[min(g, groups)], to = offsets[min(g + 1, groups)];
+        begin = max(wave_scan_max(uint32_t(min(max(from, 0), slots))), largest);
+        largest = __builtin_amdgcn_readlane(begin, 63);
+        return max(min(to, slots) - begin, 0);
     };
-    int first_begin = 0;
-    const int first_rows = load(lane, first_begin);
+    int first_begin = 0, first_largest = 0;
+    const int first_rows = load(0, first_largest, first_begin);
     int mine = (first_rows + height - 1) / height;
-    for (int g = 64 + lane; g < groups; g += 64) {
+    for (int g0 = 64, largest = first_largest; g0 < groups; g0 += 64) {
         int begin;
-        mine += (load(g, begin) + height - 1) / height;
+        mine += (load(g0, largest, begin) + height - 1) / height;
     }
     const int total = __builtin_amdgcn_readlane(wave_scan(mine), 63) * columns;
     if (index >= total) return false;
@@ -58,9 +75,9 @@ __device__ __forceinline__ bool find_tile(const int *__restrict__ offsets, int g
     const int at = index < whole ? (index & ~255) + (index % 8) * 32 + index % 256 / 8
                                  : whole + xcd_major(index - whole, total - whole);
     int before = 0;  // row tiles of the groups before this run of 64
-    for (int g0 = 0; g0 < groups; g0 += 64) {
+    for (int g0 = 0, largest = first_largest; g0 < groups; g0 += 64) {
         int begin = first_begin;
-        const int rows = g0 ? load(g0 + lane, begin) : first_rows;
+        const int rows = g0 ? load(g0, largest, begin) : first_rows;
         const int tiles = (rows + height - 1) / height;
         const int upto = before + wave_scan(tiles);
         const uint64_t past = __ballot(upto * columns > at);

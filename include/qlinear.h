@@ -368,8 +368,9 @@ int qlin_linear_noalloc(const qlin_path *path, const void *x, int ld, int src_ty
  *   order   [count]       slot -> row, ascending rows in a group; -1 from
  *                         offsets[groups] on
  *   slots   [count]       row -> slot, -1 for a row without a group
- * At most 1024 groups. The consumers hold offsets to [0, slots] in ascending
- * order and drop entries of order outside their rows. */
+ * At most 1024 groups. The consumers hold each offset to [0, slots] and to the
+ * largest before it (a slot that several groups claim is the first one's) and
+ * drop entries of order outside their rows. */
 
 /* The grouping of given ids (a stable counting sort; the same bits in every
  * run). The workspace is needed above 4096 ids. */

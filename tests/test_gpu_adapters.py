@@ -174,3 +174,31 @@ def test_two_launches(dev, dtype, rows, adapters, rank, N, K):
     run_case(dev, rows, adapters, rank, N, K, dtype, runs=rows // (adapters * 2) + 1)
     run_case(dev, rows, adapters, rank, N, K, dtype, runs=7, xpad=3, ypad=1, base="separate",
              ranks=[rank, 0, rank // 2 + 1] + [3] * (adapters - 3) if adapters > 2 else [rank, 5])
+
+
+@pytest.mark.parametrize("offsets,rows,rank,N,K", [([-5, 4, 2, 1000], 8, 8, 64, 64),
+                                                   ([40, 3, 20, 70, 60, 75], 70, 24, 80, 144),
+                                                   ([0] * 30 + [9, 2] * 20 + [33], 33, 16, 48, 48),
+                                                   ([100, 2000, 700, 3000, 5000], 2300, 40, 48, 6160)])
+def test_a_row_has_one_adapter(dev, offsets, rows, rank, N, K):
+    """Offsets out of order or out of range: a row that several adapters claim is the
+    first one's, one that none claims keeps what it held (the last case: two launches)."""
+    from breeze_tts_cpp_amd import qlinear
+    g = torch.Generator().manual_seed(rows)
+    n = len(offsets) - 1
+    held = np.maximum.accumulate(np.clip(offsets, 0, rows))
+    x, y = torch.randn(rows, K, generator=g).to(torch.bfloat16), torch.randn(rows, N, generator=g).to(torch.bfloat16)
+    a = (torch.randn(n, rank, K, generator=g) / K ** 0.5).to(torch.bfloat16)
+    b = (torch.randn(n, N, rank, generator=g) / rank ** 0.5).to(torch.bfloat16)
+    print(f"adapters offsets={offsets} rows={rows}", flush=True)
+    got = qlinear.adapter_add(x.to(dev), torch.arange(rows, dtype=torch.int32, device=dev),
+                              torch.tensor(offsets, dtype=torch.int32, device=dev), a.to(dev), b.to(dev),
+                              y.to(dev)).cpu()
+    left = np.ones(rows, bool)
+    for i in range(n):
+        at = np.arange(held[i], held[i + 1])
+        if at.size:
+            left[at] = False
+            want, bound = ref.adapter_rows(x[at], a[i], b[i], y[at], 1.0)
+            assert torch.all((got[at].double() - want).abs() <= bound), i
+    assert torch.equal(got[left].view(torch.int16), y[left].view(torch.int16))

@@ -202,3 +202,37 @@ def test_bad_indices_stay_in_bounds(dev):
     for r in (3, 0, 7, 1):
         want[r] = full[r]
     assert torch.equal(out.cpu(), want)
+
+
+# (offsets, slots): each held to [0, slots] and to the largest before it, as numpy does it below.
+@pytest.mark.parametrize("offsets,slots", [([-5, 4, 2, 1000], 8), ([0, 6, 1, 8, 3, 8], 8),
+                                           ([40, 3, 20, 70, 60, 75], 70), ([0] * 30 + [9, 2] * 20 + [33], 33),
+                                           ([64, 0] * 70 + [90], 90)])
+def test_a_slot_has_one_expert(dev, offsets, slots):
+    """Offsets out of order or out of range: a slot that several experts claim is the
+    first one's, one that none claims keeps what it held, on every tile."""
+    from breeze_tts_cpp_amd import qlinear
+    g = torch.Generator().manual_seed(len(offsets))
+    experts, N, K = len(offsets) - 1, 80, 144
+    held = np.maximum.accumulate(np.clip(offsets, 0, slots))
+    for mode, path in every_path():
+        fmt, group = MODES[mode]
+        x, sx = codes(g, slots, K, mode)
+        w, sw = zip(*[codes(g, N, K, mode) for _ in range(experts)])
+        old = torch.randn(slots, N, generator=g).to(torch.bfloat16)
+        print(f"experts {mode} offsets={offsets} slots={slots} path={path}", flush=True)
+        out = qlinear.expert_gemm(x.to(dev), sx.to(dev), torch.stack(w).to(dev), torch.stack(sw).to(dev), fmt,
+                                  torch.tensor(offsets, dtype=torch.int32, device=dev), group=group, path=path,
+                                  out=old.to(dev)).cpu()
+        left = np.ones(slots, bool)
+        for e in range(experts):
+            at = np.arange(held[e], held[e + 1])
+            if not at.size:
+                continue
+            left[at] = False
+            want = ref.expert_rows(x[at], sx[:, at] if group else sx[at], w[e], sw[e], fmt, group, torch.bfloat16)
+            if torch.is_tensor(want):
+                assert torch.equal(out[at], want), (mode, path, e)
+            else:
+                assert torch.all((out[at].double() - want[0]).abs() <= want[1]), (mode, path, e)
+        assert torch.equal(out[left].view(torch.int16), old[left].view(torch.int16))
