@@ -171,6 +171,25 @@ def _stream(stream) -> int:
     return stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream)
 
 
+def _new(shape, dtype, device, stream, returned=True):
+    """A tensor that a call on `stream` makes. Off the current stream it is memory of
+    that stream: memory of the current stream's pool may be in use by work queued
+    there before the call, and be used again there once the tensor is dropped. The
+    current stream gets to know a `returned` one, since its work may use it too."""
+    if stream is None or _stream(stream) == _stream(None):
+        return torch.empty(shape, dtype=dtype, device=device)
+    here = torch.cuda.current_stream()
+    if not isinstance(stream, torch.cuda.Stream):
+        stream = torch.cuda.ExternalStream(_stream(stream), device=here.device)
+    if stream.device != here.device:
+        raise ValueError("stream must be one of the current device")
+    with torch.cuda.stream(stream):
+        t = torch.empty(shape, dtype=dtype, device=device)
+    if returned:
+        t.record_stream(here)
+    return t
+
+
 _TYPES = {torch.bfloat16: BF16, torch.float16: F16}
 
 
@@ -185,22 +204,22 @@ def row_quantize(x: torch.Tensor, fmt: int, group: int = 0, rotation: int = 0,
         raise ValueError("quantization source must be BF16 or F16")
     rows, cols = x.shape
     if values is None:
-        values = torch.empty((rows, cols), dtype=torch.uint8, device=x.device)
+        values = _new((rows, cols), torch.uint8, x.device, stream)
     if scales is None:
         shape = ((cols + group - 1) // group, rows) if group else (rows,)
-        scales = torch.empty(shape, dtype=torch.float32, device=x.device)
+        scales = _new(shape, torch.float32, x.device, stream)
     _check(load().qlin_row_quantize(x.data_ptr(), x.stride(0), rows, cols, _TYPES[x.dtype],
                                     values.data_ptr(), scales.data_ptr(), fmt, group, rotation,
                                     _stream(stream)))
     return values, scales
 
 
-def _outputs(rows, cols, group, device, values, scales):
+def _outputs(rows, cols, group, device, values, scales, stream):
     if values is None:
-        values = torch.empty((rows, cols), dtype=torch.uint8, device=device)
+        values = _new((rows, cols), torch.uint8, device, stream)
     if scales is None:
         shape = ((cols + group - 1) // group, rows) if group else (rows,)
-        scales = torch.empty(shape, dtype=torch.float32, device=device)
+        scales = _new(shape, torch.float32, device, stream)
     return values, scales
 
 
@@ -218,7 +237,7 @@ def quantized_norm(residual: torch.Tensor, weight: torch.Tensor, fmt: int,
         if t is not None and (t.dtype != residual.dtype or not t.is_contiguous()):
             raise ValueError("quantized_norm tensors must share the residual dtype and be dense")
     rows, cols = residual.shape
-    values, scales = _outputs(rows, cols, group, residual.device, values, scales)
+    values, scales = _outputs(rows, cols, group, residual.device, values, scales, stream)
     _check(load().qlin_quantized_norm(
         residual.data_ptr(), None if update is None else update.data_ptr(),
         None if update_scale is None else update_scale.data_ptr(), weight.data_ptr(),
@@ -235,7 +254,7 @@ def quantized_gated(x: torch.Tensor, fmt: int, kind: int = 0, group: int = 0, ro
     if x.dim() != 2 or not x.is_contiguous() or x.dtype not in _TYPES or x.shape[1] % 2:
         raise ValueError("quantized_gated expects a dense [rows, 2*width] bf16/f16 tensor")
     rows, width = x.shape[0], x.shape[1] // 2
-    values, scales = _outputs(rows, width, group, x.device, values, scales)
+    values, scales = _outputs(rows, width, group, x.device, values, scales, stream)
     _check(load().qlin_quantized_gated(x.data_ptr(), _TYPES[x.dtype], rows, width, kind,
                                        values.data_ptr(), scales.data_ptr(), fmt, group,
                                        rotation, _stream(stream)))
@@ -308,13 +327,13 @@ def epilogue(bias=None, residual=None, residual_index=None, gate=None, condition
     return e
 
 
-def _quantized_out(rows, cols, group, device, values, scales):
+def _quantized_out(rows, cols, group, device, values, scales, stream):
     if values is None:
-        values = torch.empty((rows, cols), dtype=torch.uint8, device=device)
+        values = _new((rows, cols), torch.uint8, device, stream)
     if scales is None:
         groups = (cols + group - 1) // group if group else 1
         shape = (groups, rows) if group else (rows,)
-        scales = torch.empty(shape, dtype=torch.float32, device=device)
+        scales = _new(shape, torch.float32, device, stream)
     return values, scales
 
 
@@ -332,7 +351,7 @@ def norm_linear(x: torch.Tensor, wq: torch.Tensor, sw: torch.Tensor, fmt: int,
     rows, k = x.shape
     n = wq.shape[0]
     if out is None:
-        out = torch.empty((rows, n), dtype=x.dtype, device=x.device)
+        out = _new((rows, n), x.dtype, x.device, stream)
     codes, scales = encoded if encoded is not None else (None, None)
     _check(load().qlin_norm_linear(x.data_ptr(), None if fusion is None else ctypes.byref(fusion),
                                    _ptr(norm_weight), _ptr(norm_bias), _TYPES[x.dtype], rows, k,
@@ -353,7 +372,7 @@ def layer_norm_quantize(x: torch.Tensor, fmt: int, norm_weight: torch.Tensor | N
         raise ValueError("layer_norm_quantize expects a dense 2-D bf16/f16 input")
     x_rows, cols = x.shape
     rows = x_rows if rows is None else rows
-    values, scales = _quantized_out(rows, cols, group, x.device, values, scales)
+    values, scales = _quantized_out(rows, cols, group, x.device, values, scales, stream)
     _check(load().qlin_layer_norm_quantize(
         x.data_ptr(), x_rows, _TYPES[x.dtype], _ptr(norm_weight), _ptr(norm_bias), float(eps),
         None if fusion is None else ctypes.byref(fusion), _ptr(retained), rows, cols,
@@ -371,7 +390,7 @@ def pointwise_quantize(x: torch.Tensor, fmt: int, epilogue: qlin_epilogue | None
     x_rows, cols = x.shape
     if rows is None:
         rows = x_rows * (epilogue.input_repeat if epilogue is not None else 1)
-    values, scales = _quantized_out(rows, cols, group, x.device, values, scales)
+    values, scales = _quantized_out(rows, cols, group, x.device, values, scales, stream)
     _check(load().qlin_pointwise_quantize(
         x.data_ptr(), x_rows, _TYPES[x.dtype], None if epilogue is None else ctypes.byref(epilogue),
         _ptr(retained), rows, cols, values.data_ptr(), scales.data_ptr(), fmt, group, rotation,
@@ -389,7 +408,7 @@ def pointwise(x: torch.Tensor, epilogue: qlin_epilogue | None = None,
     if rows is None:
         rows = x_rows * (epilogue.input_repeat if epilogue is not None else 1)
     if out is None:
-        out = torch.empty((rows, cols), dtype=x.dtype, device=x.device)
+        out = _new((rows, cols), x.dtype, x.device, stream)
     if out.shape != (rows, cols) or out.dtype != x.dtype or not out.is_contiguous():
         raise ValueError("pointwise output must be dense [rows, cols] in the input type")
     _check(load().qlin_pointwise(
@@ -434,7 +453,7 @@ def pack_weights(wq: torch.Tensor, stream=None) -> PackedWeights:
     nbytes = int(load().qlin_packed_weight_bytes(N, K))
     if nbytes == 0:
         raise ValueError("packed weights need N % 16 == 0")
-    out = torch.empty(nbytes, dtype=torch.uint8, device=wq.device)
+    out = _new(nbytes, torch.uint8, wq.device, stream)
     _check(load().qlin_pack_weights(wq.data_ptr(), N, K, out.data_ptr(), _stream(stream)))
     return PackedWeights(out, N, K)
 
@@ -446,10 +465,10 @@ def gemm(xq: torch.Tensor, sx: torch.Tensor, wq: torch.Tensor, sw: torch.Tensor,
     M, K = xq.shape
     N = wq.shape[0]
     if out is None:
-        out = torch.empty((M, N), dtype=out_dtype, device=xq.device)
+        out = _new((M, N), out_dtype, xq.device, stream)
     need = workspace_bytes(path, M, N, K, fmt, input_group, weight_group)
     if need and workspace is None:
-        workspace = torch.empty(need, dtype=torch.uint8, device=xq.device)
+        workspace = _new(need, torch.uint8, xq.device, stream, returned=False)
     p = (path or Path()).to_c()
     ws_ptr = workspace.data_ptr() if workspace is not None else None
     ws_bytes = workspace.numel() * workspace.element_size() if workspace is not None else 0
@@ -474,12 +493,12 @@ def gemm_finish(xq: torch.Tensor, sx: torch.Tensor, wq, sw: torch.Tensor, fmt: i
     M, K = xq.shape
     N = wq.shape[0]
     if out is None:
-        out = torch.empty((M, N), dtype=out_dtype, device=xq.device)
+        out = _new((M, N), out_dtype, xq.device, stream)
     if bias is not None and (bias.dtype != out.dtype or bias.numel() != N or not bias.is_contiguous()):
         raise ValueError("finish bias must be a dense [N] tensor of the output dtype")
     need = workspace_bytes(path, M, N, K, fmt, input_group, weight_group)
     if need and workspace is None:
-        workspace = torch.empty(need, dtype=torch.uint8, device=xq.device)
+        workspace = _new(need, torch.uint8, xq.device, stream, returned=False)
     p = (path or Path()).to_c()
     ws_ptr = workspace.data_ptr() if workspace is not None else None
     ws_bytes = workspace.numel() * workspace.element_size() if workspace is not None else 0
@@ -506,14 +525,14 @@ def linear(x: torch.Tensor, wq: torch.Tensor, sw: torch.Tensor, fmt: int, group:
     rows, K = x.shape
     N = wq.shape[0]
     if out is None:
-        out = torch.empty((rows, N), dtype=out_dtype, device=x.device)
+        out = _new((rows, N), out_dtype, x.device, stream)
     if scratch is None:
         shape = ((K + group - 1) // group, rows) if group else (rows,)
-        scratch = (torch.empty((rows, K), dtype=torch.uint8, device=x.device),
-                   torch.empty(shape, dtype=torch.float32, device=x.device))
+        scratch = (_new((rows, K), torch.uint8, x.device, stream, returned=False),
+                   _new(shape, torch.float32, x.device, stream, returned=False))
     need = workspace_bytes(path, rows, N, K, fmt, group, group)
     if need and workspace is None:
-        workspace = torch.empty(need, dtype=torch.uint8, device=x.device)
+        workspace = _new(need, torch.uint8, x.device, stream, returned=False)
     ws_ptr = workspace.data_ptr() if workspace is not None else None
     ws_bytes = workspace.numel() * workspace.element_size() if workspace is not None else 0
     p = (path or Path()).to_c()
@@ -536,7 +555,7 @@ def linear_noalloc(x: torch.Tensor, wq: torch.Tensor, sw: torch.Tensor, fmt: int
     rows, K = x.shape
     N = wq.shape[0]
     if out is None:
-        out = torch.empty((rows, N), dtype=out_dtype, device=x.device)
+        out = _new((rows, N), out_dtype, x.device, stream)
     p = (path or Path()).to_c()
     _check(load().qlin_linear_noalloc(ctypes.byref(p), x.data_ptr(), x.stride(0), _TYPES[x.dtype],
                                       wq.data_ptr(), sw.data_ptr(), out.data_ptr(), rows, N, K,
@@ -574,17 +593,12 @@ def _floats(t, name, count):
 
 
 def _buffer(workspace, need, device, stream):
-    """(tensor to keep alive, pointer, bytes) of a workspace of `need` bytes. One
-    made here is the allocator's again once the call returns: a stream other
-    than the current one has to be known to it."""
+    """(tensor to keep alive, pointer, bytes) of a workspace of `need` bytes."""
     if workspace is not None:
         if workspace.get_device() != _current_device():
             _off_device()
         return workspace, workspace.data_ptr(), workspace.numel() * workspace.element_size()
-    workspace = _empty(need, dtype=torch.uint8, device=device)
-    if stream is not None:
-        workspace.record_stream(stream if isinstance(stream, torch.cuda.Stream)
-                                else torch.cuda.ExternalStream(_stream(stream), device=device))
+    workspace = _new(need, torch.uint8, device, stream, returned=False)
     return workspace, workspace.data_ptr(), need
 
 
@@ -600,13 +614,16 @@ def group_rows(ids: torch.Tensor, groups: int, order=None, slots=None, offsets=N
     if d < 0 or d != _current_device():
         _off_device()
     if order is None and slots is None and offsets is None and groups >= 0:
-        order, slots, offsets = _empty(2 * count + groups + 1, dtype=_int32, device=device) \
-            .split_with_sizes((count, count, groups + 1))
+        size = 2 * count + groups + 1
+        order, slots, offsets = \
+            (_empty(size, dtype=_int32, device=device) if stream is None
+             else _new(size, _int32, device, stream)).split_with_sizes((count, count, groups + 1))
     else:
-        order = _empty(count, dtype=_int32, device=device) if order is None \
+        order = _new(count, _int32, device, stream) if order is None \
             else _indices(order, "order", count)
-        slots = torch.empty_like(ids) if slots is None else _indices(slots, "slots", count)
-        offsets = _empty(groups + 1, dtype=_int32, device=device) if offsets is None \
+        slots = _new(ids.shape, _int32, device, stream) if slots is None \
+            else _indices(slots, "slots", count)
+        offsets = _new(groups + 1, _int32, device, stream) if offsets is None \
             else _indices(offsets, "offsets", groups + 1)
         if order.get_device() != d or slots.get_device() != d or offsets.get_device() != d:
             _off_device()
@@ -640,21 +657,23 @@ def route(logits: torch.Tensor, top_k: int, normalize: bool = False, ids=None, w
         _off_device()
     if ids is None and weights is None and order is None and slots is None and offsets is None \
             and count >= 0:
+        size = 4 * count + experts + 1
         ids, weights, order, slots, offsets = \
-            _empty(4 * count + experts + 1, dtype=_int32, device=device) \
+            (_empty(size, dtype=_int32, device=device) if stream is None
+             else _new(size, _int32, device, stream)) \
             .split_with_sizes((count, count, count, count, experts + 1))
         ids, slots = ids.view(tokens, top_k), slots.view(tokens, top_k)
         weights = weights.view(_f32).view(tokens, top_k)
     else:
-        ids = _empty((tokens, top_k), dtype=_int32, device=device) if ids is None \
+        ids = _new((tokens, top_k), _int32, device, stream) if ids is None \
             else _indices(ids, "ids", count)
-        weights = _empty((tokens, top_k), dtype=_f32, device=device) \
+        weights = _new((tokens, top_k), _f32, device, stream) \
             if weights is None else _floats(weights, "weights", count)
-        order = _empty(count, dtype=_int32, device=device) if order is None \
+        order = _new(count, _int32, device, stream) if order is None \
             else _indices(order, "order", count)
-        slots = _empty((tokens, top_k), dtype=_int32, device=device) if slots is None \
+        slots = _new((tokens, top_k), _int32, device, stream) if slots is None \
             else _indices(slots, "slots", count).view(tokens, top_k)
-        offsets = _empty(experts + 1, dtype=_int32, device=device) if offsets is None \
+        offsets = _new(experts + 1, _int32, device, stream) if offsets is None \
             else _indices(offsets, "offsets", experts + 1)
         if ids.get_device() != d or weights.get_device() != d or order.get_device() != d \
                 or slots.get_device() != d or offsets.get_device() != d:
@@ -699,7 +718,7 @@ def combine(h: torch.Tensor, slots: torch.Tensor, weights: torch.Tensor | None =
     if d < 0 or d != _current_device() or slots.get_device() != d:
         _off_device()
     if out is None:
-        out = h.new_empty((tokens, N))
+        out = h.new_empty((tokens, N)) if stream is None else _new((tokens, N), dtype, h.device, stream)
     elif out.shape != (tokens, N) or out.dtype != dtype or not out.is_contiguous():
         raise ValueError("combine output must be dense [tokens, N] in the rows' type")
     elif out.get_device() != d:
@@ -744,7 +763,8 @@ def expert_gemm(xq: torch.Tensor, sx: torch.Tensor, wq: torch.Tensor, sw: torch.
         if order.get_device() != d:
             _off_device()
     if out is None:
-        out = xq.new_empty((slots, N), dtype=out_dtype)
+        out = xq.new_empty((slots, N), dtype=out_dtype) if stream is None \
+            else _new((slots, N), out_dtype, xq.device, stream)
     kind = _TYPES.get(out.dtype)
     if kind is None or out.shape != (slots, N) or not out.is_contiguous():
         raise ValueError("expert_gemm output must be dense bf16/f16 [slots, N]")
