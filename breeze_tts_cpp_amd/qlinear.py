@@ -190,6 +190,20 @@ def _new(shape, dtype, device, stream, returned=True):
     return t
 
 
+def _buffer(workspace, need, device, stream):
+    """(tensor to keep alive, pointer, bytes) of a workspace of `need` bytes, the
+    caller's or one made here."""
+    if not need:
+        return None, None, 0
+    if workspace is None:
+        workspace = _new(need, torch.uint8, device, stream, returned=False)
+    elif not workspace.is_contiguous():  # (the library writes all bytes from its first on)
+        raise ValueError("a workspace must be a dense tensor")
+    elif workspace.get_device() != torch.cuda.current_device():
+        raise ValueError("a workspace must be on the current GPU")
+    return workspace, workspace.data_ptr(), workspace.numel() * workspace.element_size()
+
+
 _TYPES = {torch.bfloat16: BF16, torch.float16: F16}
 
 
@@ -467,11 +481,8 @@ def gemm(xq: torch.Tensor, sx: torch.Tensor, wq: torch.Tensor, sw: torch.Tensor,
     if out is None:
         out = _new((M, N), out_dtype, xq.device, stream)
     need = workspace_bytes(path, M, N, K, fmt, input_group, weight_group)
-    if need and workspace is None:
-        workspace = _new(need, torch.uint8, xq.device, stream, returned=False)
+    workspace, ws_ptr, ws_bytes = _buffer(workspace, need, xq.device, stream)
     p = (path or Path()).to_c()
-    ws_ptr = workspace.data_ptr() if workspace is not None else None
-    ws_bytes = workspace.numel() * workspace.element_size() if workspace is not None else 0
     fn = load().qlin_gemm_packed if isinstance(wq, PackedWeights) else load().qlin_gemm
     _check(fn(ctypes.byref(p), xq.data_ptr(), sx.data_ptr(), wq.data_ptr(),
                             sw.data_ptr(), out.data_ptr(), M, N, K, fmt,
@@ -497,11 +508,8 @@ def gemm_finish(xq: torch.Tensor, sx: torch.Tensor, wq, sw: torch.Tensor, fmt: i
     if bias is not None and (bias.dtype != out.dtype or bias.numel() != N or not bias.is_contiguous()):
         raise ValueError("finish bias must be a dense [N] tensor of the output dtype")
     need = workspace_bytes(path, M, N, K, fmt, input_group, weight_group)
-    if need and workspace is None:
-        workspace = _new(need, torch.uint8, xq.device, stream, returned=False)
+    workspace, ws_ptr, ws_bytes = _buffer(workspace, need, xq.device, stream)
     p = (path or Path()).to_c()
-    ws_ptr = workspace.data_ptr() if workspace is not None else None
-    ws_bytes = workspace.numel() * workspace.element_size() if workspace is not None else 0
     _check(load().qlin_gemm_finish(ctypes.byref(p), xq.data_ptr(), sx.data_ptr(), wq.data_ptr(),
                                    sw.data_ptr(), None if bias is None else bias.data_ptr(),
                                    activation, out.data_ptr(), M, N, K, fmt,
@@ -531,10 +539,7 @@ def linear(x: torch.Tensor, wq: torch.Tensor, sw: torch.Tensor, fmt: int, group:
         scratch = (_new((rows, K), torch.uint8, x.device, stream, returned=False),
                    _new(shape, torch.float32, x.device, stream, returned=False))
     need = workspace_bytes(path, rows, N, K, fmt, group, group)
-    if need and workspace is None:
-        workspace = _new(need, torch.uint8, x.device, stream, returned=False)
-    ws_ptr = workspace.data_ptr() if workspace is not None else None
-    ws_bytes = workspace.numel() * workspace.element_size() if workspace is not None else 0
+    workspace, ws_ptr, ws_bytes = _buffer(workspace, need, x.device, stream)
     p = (path or Path()).to_c()
     fn = load().qlin_linear_packed if isinstance(wq, PackedWeights) else load().qlin_linear
     _check(fn(ctypes.byref(p), x.data_ptr(), x.stride(0), _TYPES[x.dtype],
@@ -590,16 +595,6 @@ def _floats(t, name, count):
     if t.dtype != _f32 or not t.is_contiguous() or t.numel() != count:
         raise ValueError(f"{name} must be a dense f32 tensor of {count} values")
     return t
-
-
-def _buffer(workspace, need, device, stream):
-    """(tensor to keep alive, pointer, bytes) of a workspace of `need` bytes."""
-    if workspace is not None:
-        if workspace.get_device() != _current_device():
-            _off_device()
-        return workspace, workspace.data_ptr(), workspace.numel() * workspace.element_size()
-    workspace = _new(need, torch.uint8, device, stream, returned=False)
-    return workspace, workspace.data_ptr(), need
 
 
 def group_rows(ids: torch.Tensor, groups: int, order=None, slots=None, offsets=None,

@@ -182,3 +182,21 @@ def test_small_adapter_calls_need_no_workspace():
             for rank in (1, 16, 17, 32, 64, 65, 128):
                 assert K < 16 or qlinear.adapter_workspace_bytes(rows, adapters, K, rank) == 0
     assert qlinear.adapter_workspace_bytes(64, 64, 2048, 128) > 0
+
+
+def test_a_workspace_is_dense():
+    """Writes of a strided workspace's size would run into what lies between."""
+    i32 = torch.int32
+    wide = torch.zeros(1 << 16, 2, dtype=torch.uint8)
+    ids = torch.zeros(5000, dtype=i32)
+    x, sx = torch.zeros(8, 4096, dtype=torch.uint8), torch.zeros(8)
+    w, sw = torch.zeros(16, 4096, dtype=torch.uint8), torch.zeros(16)
+    path = qlinear.Path(qlinear.KIND_SKINNY, 16, 16, 2, 8)
+    assert qlinear.workspace_bytes(path, 8, 16, 4096, I8) > 0
+    for call in (lambda ws: qlinear.gemm(x, sx, w, sw, I8, path=path, workspace=ws),
+                 lambda ws: qlinear.gemm_finish(x, sx, w, sw, I8, path=path, workspace=ws),
+                 lambda ws: qlinear.linear(x.view(torch.bfloat16), w[:, :2048].contiguous(), sw, I8, path=path,
+                                           scratch=(x, sx), workspace=ws),
+                 lambda ws: qlinear._buffer(ws, 1 << 16, ids.device, None)):
+        with pytest.raises(ValueError, match="dense"):
+            call(wide[:, 0])
