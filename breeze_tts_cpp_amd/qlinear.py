@@ -584,6 +584,11 @@ def _off_device():
     raise ValueError("operands must be on one GPU, the current one")
 
 
+def _too_large():
+    # (ctypes passes the low 32 bits of a larger int: another call.)
+    raise ValueError("sizes and strides must be below 2^31")
+
+
 def _indices(t, name, count=None):
     if t.dtype != _int32 or not t.is_contiguous() or (count is not None and t.numel() != count):
         raise ValueError(f"{name} must be a dense int32 tensor"
@@ -605,6 +610,8 @@ def group_rows(ids: torch.Tensor, groups: int, order=None, slots=None, offsets=N
     L = _lib or load()
     _indices(ids, "ids")
     count, device = ids.numel(), ids.device
+    if (count | groups) >> 31 > 0:
+        _too_large()
     d = ids.get_device()
     if d < 0 or d != _current_device():
         _off_device()
@@ -645,8 +652,10 @@ def route(logits: torch.Tensor, top_k: int, normalize: bool = False, ids=None, w
     ld, unit = logits.stride()
     if unit != 1 and experts > 1:
         raise ValueError("route expects 2-D f32/bf16/f16 logits with unit column stride")
-    if tokens == 1 and ld < experts:
+    if tokens == 1:
         ld = experts
+    if (tokens | experts | ld | top_k) >> 31 > 0:
+        _too_large()
     count, device, d = tokens * top_k, logits.device, logits.get_device()
     if d < 0 or d != _current_device():
         _off_device()
@@ -698,6 +707,8 @@ def combine(h: torch.Tensor, slots: torch.Tensor, weights: torch.Tensor | None =
         raise ValueError("combine expects dense int32 slots [tokens, top_k]")
     tokens, top_k = slots.shape
     h_rows, N = h.shape
+    if (tokens | top_k | h_rows | N) >> 31 > 0:
+        _too_large()
     w_ptr = base_ptr = None
     if weights is not None:
         _floats(weights, "weights", tokens * top_k)
@@ -757,6 +768,8 @@ def expert_gemm(xq: torch.Tensor, sx: torch.Tensor, wq: torch.Tensor, sw: torch.
         slots, order_ptr = _indices(order, "order").numel(), order.data_ptr()
         if order.get_device() != d:
             _off_device()
+    if (x_rows | K | experts | N | slots | divisor) >> 31 > 0:
+        _too_large()
     if out is None:
         out = xq.new_empty((slots, N), dtype=out_dtype) if stream is None \
             else _new((slots, N), out_dtype, xq.device, stream)
@@ -810,6 +823,8 @@ def adapter_add(x: torch.Tensor, order: torch.Tensor, offsets: torch.Tensor, a: 
     elif base.shape != shape or base.dtype != dtype or (base.stride(1) != 1 and N > 1) \
             or (rows > 1 and base.stride(0) != ldy) or base.get_device() != d:
         raise ValueError("adapter_add base must be rows like the output's, of one stride")
+    if (rows | K | adapters | N | rank | ldx | ldy) >> 31 > 0:
+        _too_large()
     ranks_ptr = scales_ptr = ws_ptr = None
     if ranks is not None:
         ranks_ptr = _indices(ranks, "ranks", adapters).data_ptr()

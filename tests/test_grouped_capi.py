@@ -200,3 +200,33 @@ def test_a_workspace_is_dense():
                  lambda ws: qlinear._buffer(ws, 1 << 16, ids.device, None)):
         with pytest.raises(ValueError, match="dense"):
             call(wide[:, 0])
+
+
+def test_sizes_past_32_bits():
+    """Sizes and strides whose low 32 bits would be another, valid call."""
+    i32, bf = torch.int32, torch.bfloat16
+    meta = lambda *s, dtype=i32: torch.empty(*s, dtype=dtype, device="meta")
+    far = (1 << 32) + 8
+    u8, f32 = torch.uint8, torch.float32
+    calls = [
+        lambda: qlinear.group_rows(meta(far), 4),
+        lambda: qlinear.group_rows(meta(8), far),
+        lambda: qlinear.route(meta(far, 16, dtype=bf), 2),
+        lambda: qlinear.route(meta(2, 16, dtype=bf).as_strided((2, 16), (far, 1)), 2),
+        lambda: qlinear.route(meta(2, 16, dtype=bf), far),
+        lambda: qlinear.combine(meta(far, 16, dtype=bf), meta(4, 2)),
+        lambda: qlinear.combine(meta(8, 16, dtype=bf), meta(far, 2)),
+        lambda: qlinear.expert_gemm(meta(far, 16, dtype=u8), meta(far, dtype=f32), meta(2, 16, 16, dtype=u8),
+                                    meta(2, 16, dtype=f32), I8, meta(3)),
+        lambda: qlinear.expert_gemm(meta(8, 16, dtype=u8), meta(8, dtype=f32), meta(2, 16, 16, dtype=u8),
+                                    meta(2, 16, dtype=f32), I8, meta(3), order=meta(far)),
+        lambda: qlinear.expert_gemm(meta(8, 16, dtype=u8), meta(8, dtype=f32), meta(2, 16, 16, dtype=u8),
+                                    meta(2, 16, dtype=f32), I8, meta(3), order=meta(8), divisor=far),
+        lambda: qlinear.adapter_add(meta(far, 16, dtype=bf), meta(far), meta(3), meta(2, 8, 16, dtype=bf),
+                                    meta(2, 16, 8, dtype=bf), meta(far, 16, dtype=bf)),
+        lambda: qlinear.adapter_add(meta(4, 16, dtype=bf), meta(4), meta(3), meta(2, 8, 16, dtype=bf),
+                                    meta(2, 16, 8, dtype=bf), meta(4, 16, dtype=bf).as_strided((4, 16), (far, 1))),
+    ]
+    for i, call in enumerate(calls):
+        with pytest.raises(ValueError, match="2.31"):
+            call()
