@@ -222,6 +222,10 @@ int qlin_combine(const void *h, int h_rows, const int *slots, const float *weigh
         return fail(QLIN_ERR_INVALID, "combine output overlaps its input rows");
     if (base && base != out && overlap(base, size_t(tokens) * N * 2, out, size_t(tokens) * N * 2))
         return fail(QLIN_ERR_INVALID, "combine output overlaps part of its base");
+    const size_t choices = size_t(tokens) * top_k * 4;
+    if (overlap(slots, choices, out, size_t(tokens) * N * 2) ||
+        (weights && overlap(weights, choices, out, size_t(tokens) * N * 2)))
+        return fail(QLIN_ERR_INVALID, "combine output overlaps its slots or weights");
     qlin::launch_combine({h, slots, weights, base, out, h_rows, tokens, top_k, N, type},
                          reinterpret_cast<hipStream_t>(stream));
     return check_launch("combine launch");

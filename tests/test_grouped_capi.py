@@ -230,3 +230,21 @@ def test_sizes_past_32_bits():
     for i, call in enumerate(calls):
         with pytest.raises(ValueError, match="2.31"):
             call()
+
+
+OUT = FAR * 20  # of a call's output; the other arrays far from it and from each other
+
+
+def refuses_overlaps(call, at, size, arrays):
+    """Each of `arrays` (argument -> bytes) on the first and on the last 16 bytes of the
+    `size` bytes that the call writes at `at`."""
+    for name, n in arrays.items():
+        for where in (at - (n - 1) // 16 * 16, at + (size - 1) // 16 * 16):
+            assert call(**{name: where}) == -1 and b"overlap" in qlinear.load().qlin_last_error(), (name, where)
+
+
+def test_combine_output_is_apart():
+    def call(h=FAR, slots=SLOTS, w=WEIGHTS, base=None):
+        return qlinear.load().qlin_combine(h, 8, slots, w, base, OUT, 40, 2, 64, BF16, None)
+
+    refuses_overlaps(call, OUT, 40 * 64 * 2, {"h": 8 * 64 * 2, "slots": 40 * 2 * 4, "w": 40 * 2 * 4})
