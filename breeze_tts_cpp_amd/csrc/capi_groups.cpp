@@ -286,6 +286,11 @@ int qlin_expert_gemm(const qlin_path *path, const void *x, const float *sx, int 
     if (qlin::expert_row_tiles(slots, experts, t.tokens) * ((long(N) + t.channels - 1) / t.channels) >
         INT32_MAX)
         return fail(QLIN_ERR_UNSUPPORTED, "grouped GEMM has more than 2^31 - 1 macro tiles");
+    const size_t y_bytes = size_t(slots) * N * 2, blocks = group ? (size_t(K) + 127) / 128 : 1;
+    if (overlap(sx, blocks * x_rows * 4, y, y_bytes) || overlap(w, size_t(experts) * N * K, y, y_bytes) ||
+        overlap(sw, blocks * experts * N * 4, y, y_bytes) || overlap(offsets, size_t(experts + 1) * 4, y, y_bytes) ||
+        (order && overlap(order, size_t(slots) * 4, y, y_bytes)))
+        return fail(QLIN_ERR_INVALID, "grouped GEMM output overlaps its weights, scales or indices");
     qlin::ExpertArgs a{static_cast<const uint8_t *>(x), sx, order, offsets,
                        static_cast<const uint8_t *>(w), sw, y, x_rows, divisor, scatter != 0,
                        experts, slots, N, K, fmt, out_type, group};

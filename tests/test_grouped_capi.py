@@ -248,3 +248,16 @@ def test_combine_output_is_apart():
         return qlinear.load().qlin_combine(h, 8, slots, w, base, OUT, 40, 2, 64, BF16, None)
 
     refuses_overlaps(call, OUT, 40 * 64 * 2, {"h": 8 * 64 * 2, "slots": 40 * 2 * 4, "w": 40 * 2 * 4})
+
+
+@pytest.mark.parametrize("group,blocks", [(0, 1), (128, 3)])
+def test_expert_output_is_apart(group, blocks):
+    rows, slots, experts, N, K = 24, 40, 8, 64, 272
+
+    def call(x=FAR, sx=FAR * 2, order=FAR * 3, off=FAR * 4, w=FAR * 5, sw=FAR * 6):
+        return qlinear.load().qlin_expert_gemm(None, x, sx, rows, order, 2, off, w, sw, experts, OUT, 0, slots,
+                                               N, K, I8, BF16, group, None)
+
+    refuses_overlaps(call, OUT, slots * N * 2,
+                     {"x": rows * K, "sx": blocks * rows * 4, "order": slots * 4, "off": (experts + 1) * 4,
+                      "w": experts * N * K, "sw": blocks * experts * N * 4})
