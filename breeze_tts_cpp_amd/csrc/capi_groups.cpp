@@ -46,6 +46,14 @@ bool rows_overlap(const void *a, int lda, int an, const void *b, int ldb, int bn
     return column < an || column + bn > lda;
 }
 
+// The rows [a, a + an) of stride lda (16-bit elements) and the bytes [b, b + bn) share one; an
+// array that lies between two rows does not.
+bool rows_overlap_bytes(const void *a, int lda, int an, int rows, const void *b, size_t bn) {
+    if (!b || !overlap(a, (size_t(rows - 1) * lda + an) * 2, b, bn)) return false;
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b), row = size_t(lda) * 2;
+    return y < x || (y - x) % row < size_t(an) * 2 || (y - x) % row + bn > row;
+}
+
 // Most ids of one grouping (index arithmetic past the last run stays in int).
 constexpr int kMaxIds = 1 << 30;
 
@@ -341,6 +349,20 @@ int qlin_adapter_add(const void *x, int ldx, const int *order, const int *offset
         return fail(QLIN_ERR_UNSUPPORTED, "adapter input rows exceed 2 GiB");
     if (qlin::expert_row_tiles(rows, adapters, 16) * ((long(N) + 255) / 256) > INT32_MAX)
         return fail(QLIN_ERR_UNSUPPORTED, "adapter call has more than 2^31 - 1 tiles");
+    const struct { const void *p; size_t bytes; } inputs[] = {
+        {a, size_t(adapters) * rank * K * 2}, {b, size_t(adapters) * N * rank * 2},
+        {order, size_t(rows) * 4}, {offsets, size_t(adapters + 1) * 4},
+        {ranks, size_t(adapters) * 4}, {scales, size_t(adapters) * 4}};
+    for (const auto &in : inputs) {
+        if (rows_overlap_bytes(y, ldy, N, rows, in.p, in.bytes))
+            return fail(QLIN_ERR_INVALID, "adapter output overlaps its matrices or index arrays");
+        if (need && in.p && overlap(workspace, need, in.p, in.bytes))
+            return fail(QLIN_ERR_INVALID, "adapter workspace overlaps its matrices or index arrays");
+    }
+    if (need && (rows_overlap_bytes(y, ldy, N, rows, workspace, need) ||
+                 rows_overlap_bytes(x, ldx, K, rows, workspace, need) ||
+                 (base && rows_overlap_bytes(base, ldy, N, rows, workspace, need))))
+        return fail(QLIN_ERR_INVALID, "adapter workspace overlaps its rows");
     qlin::launch_adapter({x, order, offsets, a, b, ranks, scales, base, y, ldx, ldy, rows, adapters,
                           rank, N, K, type, workspace},
                          reinterpret_cast<hipStream_t>(stream));

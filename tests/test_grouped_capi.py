@@ -261,3 +261,34 @@ def test_expert_output_is_apart(group, blocks):
     refuses_overlaps(call, OUT, slots * N * 2,
                      {"x": rows * K, "sx": blocks * rows * 4, "order": slots * 4, "off": (experts + 1) * 4,
                       "w": experts * N * K, "sw": blocks * experts * N * 4})
+
+
+def adapter_call(rows, n, rank, N, K, ldy, ws=None, wsb=0):
+    def call(x=FAR, order=FAR * 2, off=FAR * 3, a=FAR * 4, b=FAR * 5, ranks=FAR * 6, scales=FAR * 7, base=FAR * 8,
+             y=OUT, ws=ws):
+        return qlinear.load().qlin_adapter_add(x, K, order, off, rows, n, a, b, rank, ranks, scales, base, y, ldy,
+                                               N, K, BF16, ws, wsb, None)
+    return call
+
+
+def test_adapter_output_is_apart():
+    rows, n, rank, N, K = 40, 3, 16, 64, 256
+    sizes = {"order": rows * 4, "off": (n + 1) * 4, "a": n * rank * K * 2, "b": n * N * rank * 2, "ranks": n * 4,
+             "scales": n * 4}
+    refuses_overlaps(adapter_call(rows, n, rank, N, K, N), OUT, rows * N * 2, sizes)
+    # A column range of wider rows: whatever reaches from the gap into a row, or spans one.
+    call = adapter_call(rows, n, rank, N, K, N + 32)
+    refuses_overlaps(call, OUT, ((rows - 1) * (N + 32) + N) * 2, sizes)
+    for name in ("off", "ranks", "scales"):
+        for at in (OUT + N * 2 - 4, OUT + (N + 32) * 2 - 4):
+            assert call(**{name: at}) == -1 and b"overlap" in qlinear.load().qlin_last_error(), (name, at)
+
+
+def test_adapter_workspace_is_apart():
+    rows, n, rank, N, K = 4096, 4, 64, 64, 6144
+    need = qlinear.adapter_workspace_bytes(rows, n, K, rank)
+    assert need > 0
+    call = adapter_call(rows, n, rank, N, K, N, FAR * 30, need)
+    refuses_overlaps(call, FAR * 30, need,
+                     {"order": rows * 4, "off": (n + 1) * 4, "a": n * rank * K * 2, "b": n * N * rank * 2,
+                      "ranks": n * 4, "scales": n * 4, "x": rows * K * 2, "base": rows * N * 2, "y": rows * N * 2})
