@@ -80,6 +80,10 @@ int check_grouping(const char *what, const int *ids, long count, int groups, con
                     workspace ? bytes : size_t(0));
     if (need && !aligned(workspace, 4))
         return fail(QLIN_ERR_ALIGNMENT, "%s: workspace must be 4-byte aligned", what);
+    // (The placing launch reads the counts there while it writes order and slots.)
+    for (const auto &a : arrays)
+        if (need && overlap(workspace, need, a.p, a.bytes))
+            return fail(QLIN_ERR_INVALID, "%s: workspace overlaps ids, order, slots or offsets", what);
     return QLIN_OK;
 }
 
@@ -206,6 +210,9 @@ int qlin_route(const void *logits, int ld, int logits_type, int tokens, int expe
             return fail(QLIN_ERR_INVALID, "router outputs overlap its logits or each other");
     if (overlap(weights, flat, logits, logits_bytes))
         return fail(QLIN_ERR_INVALID, "router outputs overlap its logits or each other");
+    const size_t need = qlin::group_workspace_bytes(tokens * top_k, experts);
+    if (need && (overlap(workspace, need, logits, logits_bytes) || overlap(workspace, need, weights, flat)))
+        return fail(QLIN_ERR_INVALID, "router workspace overlaps its logits or weights");
     qlin::launch_route({logits, ld, logits_type, tokens, experts, top_k, normalize != 0, ids, weights},
                        {ids, tokens * top_k, experts, order, slots, offsets, workspace},
                        reinterpret_cast<hipStream_t>(stream));

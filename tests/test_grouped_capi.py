@@ -292,3 +292,21 @@ def test_adapter_workspace_is_apart():
     refuses_overlaps(call, FAR * 30, need,
                      {"order": rows * 4, "off": (n + 1) * 4, "a": n * rank * K * 2, "b": n * N * rank * 2,
                       "ranks": n * 4, "scales": n * 4, "x": rows * K * 2, "base": rows * N * 2, "y": rows * N * 2})
+
+
+def test_grouping_workspace_is_apart():
+    L = qlinear.load()
+    count, groups, at = 5000, 40, FAR * 30
+    need = L.qlin_group_rows_workspace_bytes(count, groups)
+
+    def rows(ids=IDS, order=ORDER, slots=SLOTS, offsets=OFFSETS):
+        return L.qlin_group_rows(ids, count, groups, order, slots, offsets, at, need, None)
+
+    index = {"ids": count * 4, "order": count * 4, "slots": count * 4, "offsets": (groups + 1) * 4}
+    refuses_overlaps(rows, at, need, index)
+
+    def route(logits=FAR * 20, ids=IDS, weights=WEIGHTS, order=ORDER, slots=SLOTS, offsets=OFFSETS):
+        return L.qlin_route(logits, groups, F32, count // 4, groups, 4, 0, ids, weights, order, slots, offsets, at,
+                            need, None)
+
+    refuses_overlaps(route, at, need, {**index, "weights": count * 4, "logits": count // 4 * groups * 4})
