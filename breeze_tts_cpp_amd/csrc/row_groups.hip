@@ -167,7 +167,8 @@ __device__ __forceinline__ void place_ids(const GroupArgs &a, int begin, int end
         const int rank = __builtin_popcountll(same & ((1ull << lane) - 1));
         const int slot = valid ? next[id] + rank : -1;
         if (i < end) a.slots[i] = slot;
-        if (valid) a.order[slot] = i;
+        // (Always within the ids, unless another call writes the same workspace or ids meanwhile.)
+        if (uint32_t(slot) < uint32_t(a.count)) a.order[slot] = i;
         if (valid && rank == 0) next[id] = slot + __builtin_popcountll(same);
         __builtin_amdgcn_wave_barrier();
     }
