@@ -408,11 +408,16 @@ int qlin_combine(const void *h, int h_rows, const int *slots, const float *weigh
  * `slots` is the capacity of the grouping (the ids' count): offsets say how
  * many are in use. A router's first product gathers (order, divisor = top_k),
  * its second reads slots (order NULL); heads or codebooks gather and scatter
- * (divisor 1). Scaling and shape rules are qlin_gemm's: (acc * sx) * sw, or
- * fma(p_g, sx_g * sw_g, r) over ascending K groups of each K slice. Gathered
- * rows must lie in 2 GiB (x_rows * K). `path` may be NULL (planned as
- * qlin_expert_plan: by slots / experts); its tiles are those that plans of
- * some shape give. */
+ * (divisor 1; `order` names a row at most once there, or any one of the row's
+ * results is kept). Scaling is qlin_gemm's: (acc * sx) * sw, or
+ * fma(p_g, sx_g * sw_g, r) over ascending K groups of each K slice. K and N are
+ * multiples of 16, K groups are of 128 only, and weights are row-major: there is
+ * no grouped form of groups of 32 or 64, of packed weights or of the finish.
+ * Gathered rows must lie in 2 GiB (x_rows * K). `path` may be NULL (planned as
+ * qlin_expert_plan: by the mean slots / experts, since the groups' sizes are on the
+ * device; where nearly all rows fall to few experts a path of more tokens, such as
+ * the plan for fewer experts, is faster); its tiles are those that plans of some
+ * shape give. */
 int qlin_expert_plan(int slots, int experts, int N, int K, int fmt, int group, qlin_path *path);
 int qlin_expert_gemm(const qlin_path *path, const void *x, const float *sx, int x_rows,
                      const int *order, int divisor, const int *offsets, const void *w,
