@@ -54,6 +54,9 @@ bool rows_overlap_bytes(const void *a, int lda, int an, int rows, const void *b,
     return y < x || (y - x) % row < size_t(an) * 2 || (y - x) % row + bn > row;
 }
 
+// A launch has fewer than 2^32 threads.
+bool grid_fits(long workgroups, long threads) { return workgroups <= long(UINT32_MAX) / threads; }
+
 // Most ids of one grouping (index arithmetic past the last run stays in int).
 constexpr int kMaxIds = 1 << 30;
 
@@ -201,6 +204,9 @@ int qlin_route(const void *logits, int ld, int logits_type, int tokens, int expe
     const int status = check_grouping("router", ids, long(tokens) * top_k, experts, order, slots,
                                       offsets, workspace, workspace_bytes);
     if (status) return status;
+    const long each = 256 / (experts <= 128 ? 16 : 64);  // tokens a workgroup
+    if (!grid_fits((tokens + each - 1) / each, 256))
+        return fail(QLIN_ERR_UNSUPPORTED, "router grid exceeds capacity");
     const size_t logits_bytes = (size_t(tokens - 1) * ld + experts) * (logits_type == QLIN_F32 ? 4 : 2);
     const size_t flat = size_t(tokens) * top_k * 4, index_bytes[] = {flat, flat, flat, size_t(experts + 1) * 4};
     const void *index[] = {ids, order, slots, offsets};
@@ -227,7 +233,7 @@ int qlin_combine(const void *h, int h_rows, const int *slots, const float *weigh
     if (h_rows < 1 || tokens < 1 || top_k < 1 || top_k > qlin::kMaxTopK || N < 1)
         return fail(QLIN_ERR_INVALID, "combine shape h_rows=%d tokens=%d top_k=%d N=%d", h_rows,
                     tokens, top_k, N);
-    if (long(tokens) * ((long(N) + 2047) / 2048) > INT32_MAX)
+    if (!grid_fits(long(tokens) * ((long(N) + 2047) / 2048), 256))
         return fail(QLIN_ERR_INVALID, "combine grid exceeds capacity");
     if (!h || !slots || !out) return fail(QLIN_ERR_INVALID, "combine: null pointer");
     if (!aligned(h, 2) || !aligned(base, 2) || !aligned(out, 2) || !aligned(slots, 4) ||
@@ -298,9 +304,9 @@ int qlin_expert_gemm(const qlin_path *path, const void *x, const float *sx, int 
     const auto &t = qlin::kExpertTiles[tile];
     if (long(t.channels > t.tokens ? t.channels : t.tokens) * K > INT32_MAX)
         return fail(QLIN_ERR_UNSUPPORTED, "grouped GEMM tile rows exceed 2 GiB");
-    if (qlin::expert_row_tiles(slots, experts, t.tokens) * ((long(N) + t.channels - 1) / t.channels) >
-        INT32_MAX)
-        return fail(QLIN_ERR_UNSUPPORTED, "grouped GEMM has more than 2^31 - 1 macro tiles");
+    if (!grid_fits(qlin::expert_row_tiles(slots, experts, t.tokens) * ((long(N) + t.channels - 1) / t.channels),
+                   64 * t.waves))
+        return fail(QLIN_ERR_UNSUPPORTED, "grouped GEMM has too many macro tiles for a launch");
     const size_t y_bytes = size_t(slots) * N * 2, blocks = group ? (size_t(K) + 127) / 128 : 1;
     if (overlap(sx, blocks * x_rows * 4, y, y_bytes) || overlap(w, size_t(experts) * N * K, y, y_bytes) ||
         overlap(sw, blocks * experts * N * 4, y, y_bytes) || overlap(offsets, size_t(experts + 1) * 4, y, y_bytes) ||
@@ -354,8 +360,10 @@ int qlin_adapter_add(const void *x, int ldx, const int *order, const int *offset
     // Rows of x and an adapter's a are addressed through 32-bit buffer ranges.
     if (x_bytes > size_t(INT32_MAX) || size_t(rank) * K * 2 > size_t(INT32_MAX))
         return fail(QLIN_ERR_UNSUPPORTED, "adapter input rows exceed 2 GiB");
-    if (qlin::expert_row_tiles(rows, adapters, 16) * ((long(N) + 255) / 256) > INT32_MAX)
-        return fail(QLIN_ERR_UNSUPPORTED, "adapter call has more than 2^31 - 1 tiles");
+    // (The second of two launches, up to rank 64: 32 rows and 256 channels a workgroup. Other
+    // forms take more channels where the rows are many.)
+    if (need && rank <= 64 && !grid_fits(qlin::expert_row_tiles(rows, adapters, 32) * ((long(N) + 255) / 256), 512))
+        return fail(QLIN_ERR_UNSUPPORTED, "adapter call has too many tiles for a launch");
     const struct { const void *p; size_t bytes; } inputs[] = {
         {a, size_t(adapters) * rank * K * 2}, {b, size_t(adapters) * N * rank * 2},
         {order, size_t(rows) * 4}, {offsets, size_t(adapters + 1) * 4},

@@ -310,3 +310,28 @@ def test_grouping_workspace_is_apart():
                             need, None)
 
     refuses_overlaps(route, at, need, {**index, "weights": count * 4, "logits": count // 4 * groups * 4})
+
+
+def test_grids_past_a_launch():
+    """2^32 threads and more are refused before the launch."""
+    L = qlinear.load()
+    assert L.qlin_combine(FAR, 8, FAR * 2, None, None, OUT, 1 << 24, 1, 8, BF16, None) == -1
+    assert b"capacity" in L.qlin_last_error()
+    for tokens, experts in (((1 << 28) - 1, 2), ((1 << 26) - 1, 129)):
+        need = L.qlin_group_rows_workspace_bytes(tokens, experts)
+        assert L.qlin_route(FAR * 20, experts, BF16, tokens, experts, 1, 0, IDS, WEIGHTS, ORDER, SLOTS, OFFSETS,
+                            FAR * 30, need, None) == -4
+        assert b"capacity" in L.qlin_last_error()
+    # 32-token tiles of 64 channels, four waves: 2^24 of them
+    assert qlinear.expert_plan(1 << 10, 1 << 9, 1 << 16, 128, I8) == qlinear.Path(qlinear.KIND_TILED, 32, 64, 1, 4)
+    rows, N = 1 << 14, 1 << 21
+    path = qlinear.Path(qlinear.KIND_TILED, 32, 64, 1, 4)
+    assert L.qlin_expert_gemm(ctypes.byref(path.to_c()), FAR, FAR * 2, rows, None, 1, FAR * 3, FAR * 4, FAR * 5, 1,
+                              OUT, 0, rows, N, 16, I8, BF16, 0, None) == -4
+    assert b"tiles" in L.qlin_last_error()
+    rows, N, rank = 1 << 20, 1 << 16, 64
+    need = qlinear.adapter_workspace_bytes(rows, 1, 16, rank)
+    assert need > 0
+    assert L.qlin_adapter_add(FAR, 16, FAR * 2, FAR * 3, rows, 1, FAR * 4, FAR * 5, rank, None, None, None, OUT, N,
+                              N, 16, BF16, FAR * 30, need, None) == -4
+    assert b"tiles" in L.qlin_last_error()
