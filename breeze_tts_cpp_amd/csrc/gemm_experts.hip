@@ -15,11 +15,15 @@
 // summed through LDS in ascending slice order.
 //
 // Bound by the live experts' weights while an expert has few rows (192 slots of 64
-// experts, 2048 x 1024 FP8: 20.9 us, 5.3 TB/s with what the Infinity Cache gives; 8 of 64, 2048 x
-// 2048 INT8: 7.6 us, 4.4 TB/s), by the MFMAs and short last tiles with many (16384 slots of 32
-// experts, 4096 x 2048 INT8: 158 us, 1.74 POPS; 4096 rows each 2.0), between them
-// by each workgroup's chain of offsets, first stages and stores beside the rows through L2 (8000
-// slots of 64, 2048 x 1024 FP8 with K groups: 52.6 us, 640 TFLOPS; 42 without its loads).
+// experts, 2048 x 1024 FP8: 21.6 us, 5.2 TB/s with what the Infinity Cache gives; 8 of 64, 2048 x
+// 2048 INT8: 7.7 us, 4.4 TB/s). With many no part alone is the bound: 16384 slots of 32
+// experts, 4096 x 2048 INT8, take 158 us where the routing's tiles fill five rounds of
+// workgroups, 178-186 where they begin a sixth (1.5-1.74 POPS; 2.0 at 4096 rows each). Of 167
+// us on average 142 stay without the MFMAs, 136 without the loads past the first stages, 155
+// without fragment reads or without stores, 85 without MFMAs and loads, 58 with prologue,
+// barriers and epilogue alone. Between them a workgroup's fixed part is the most (7680 slots of
+// 64, 2048 x 1024 FP8 with K groups, 57 us, 570 TFLOPS: 53 without MFMAs, fragment reads or
+// stores, 43 without the loads past the first stages, 27 without the walk over K).
 #include "qlin_device.hpp"
 #include "qlin_internal.hpp"
 #include "row_groups.hpp"
