@@ -128,3 +128,42 @@ def test_the_current_stream_by_its_handle(dev, calls):
         want = [bits(t) for t in tensors(calls[name](None))]
         for s in (torch.cuda.current_stream(), torch.cuda.current_stream().cuda_stream):
             assert all(torch.equal(a, bits(t)) for a, t in zip(want, tensors(calls[name](s))))
+
+
+def test_the_default_stream_from_another(dev, calls):
+    """The default stream as the argument, by object and by its handle (0), while another is current."""
+    here = torch.cuda.Stream()
+    for name in ("linear", "route", "combine", "adapter_add"):
+        want = [bits(t) for t in tensors(calls[name](None))]
+        torch.cuda.synchronize()
+        for s in (torch.cuda.default_stream(), 0):
+            with torch.cuda.stream(here):
+                got = tensors(calls[name](s))
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, bits(t)) for a, t in zip(want, got)), name
+
+
+@pytest.mark.parametrize("name", ["linear", "gemm_split", "route", "expert_gemm", "adapter_add"])
+def test_forked_in_a_graph(dev, calls, name):
+    """Captured on a stream that forks from the capturing one and joins it again; what the
+    call makes lives in the graph's pool."""
+    want = [bits(t) for t in tensors(calls[name](None))]
+    main, fork = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=main):
+        fork.wait_stream(main)
+        first = tensors(calls[name](fork))
+        second = tensors(calls[name](fork))
+        main.wait_stream(fork)
+    torch.cuda.synchronize()
+    for _ in range(4):
+        for t in first + second:
+            t.zero_()
+        junk = torch.full((1 << 20,), 5, dtype=torch.int32, device=dev)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        for outs in (first, second):
+            assert all(torch.equal(a, bits(t)) for a, t in zip(want, outs))
+        del junk
